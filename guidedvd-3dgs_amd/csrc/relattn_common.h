@@ -1,0 +1,66 @@
+// relattn_common.h -- shared by relattn_forward.hip and relattn_backward.hip: the bias by distance, the geometry of a call.
+#pragma once
+#include "../../include/gvd_relattn.h"
+#include "diffusion_common.h"
+
+namespace gvdr {
+
+using namespace gvdd;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -3.4028234e38f;   // the running maximum before a row has seen anything: below every score that is not -infinity
+
+// What every kernel of a call reads.  `first` by value: a few hundred bytes of kernel arguments, nothing on the device to keep or to upload.
+struct Geo {
+    int H, Nq, Nk, buckets, side, both, causal, reach, q_start, table_type;
+    float scale, c, inv_scale;             // c = scale log2(e)
+    const int* q_starts;
+    const int* kv_lens;
+    const void* table;
+    long long q_bs, q_rs, kv_bs, kv_rs, o_bs, o_rs;
+    int first[GVD_RELATTN_MAX_SIDE];
+};
+
+// The bias by distance lies in LDS for distances -reach - PAD .. reach + PAD: a block of 64 keys x 32 queries spans 95 distances, so a block with one
+// distance inside (-reach, reach) reads no further.  Blocks without one have a single bias.
+constexpr int PAD = 95;
+__host__ __device__ inline int bias_len(int reach) { return 2 * (reach + PAD) + 1; }
+
+__device__ __forceinline__ int bucket_of(const Geo& g, int d)
+{
+    const int n = g.both ? (d < 0 ? -d : d) : (d < 0 ? -d : 0);
+    int b = -1;
+    for (int k = 0; k < g.side; k++) b += g.first[k] <= n;
+    return b + (g.both && d > 0 ? g.side : 0);
+}
+
+__device__ __forceinline__ float table_at(const Geo& g, int bucket, int h)
+{
+    const int i = bucket * g.H + h;
+    if (g.table_type == 0) return ((const float*)g.table)[i];
+    if (g.table_type == 1) return (float)((const _Float16*)g.table)[i];
+    return (float)((const __bf16*)g.table)[i];
+}
+
+// The bias as the products' accumulators start from it: over the scale, so that scores come out of the matrix unit as (q.k + bias / scale).  Entries at or below
+// -10000 mask their bucket, as -infinity does: among them are the lowest values of every type and the constants used in their place, and a score that
+// far out would leave 32 bits nothing for q.k.  For the same reason an entry counts as 10000 at most.
+__device__ __forceinline__ float start_value(const Geo& g, float bias)
+{
+    return (bias <= -10000.f ? -INFINITY : (bias > 10000.f ? 10000.f : bias)) * g.inv_scale;
+}
+
+__device__ __forceinline__ void fill_bias(const Geo& g, int h, float* sBias, int tid, int nt)
+{
+    for (int e = tid; e < bias_len(g.reach); e += nt) sBias[e] = start_value(g, table_at(g, bucket_of(g, e - g.reach - PAD), h));
+}
+
+__device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+__device__ __forceinline__ int len_of(const Geo& g, int b) { return g.kv_lens ? clamp_int(g.kv_lens[b], 0, g.Nk) : g.Nk; }
+__device__ __forceinline__ int start_of(const Geo& g, int b) { return clamp_int(g.q_starts ? g.q_starts[b] : g.q_start, -(1 << 29), 1 << 29); }
+
+// Host side: checks a problem and fills a Geo (the table's pointer aside).
+int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who);
+int compute_units();
+
+}  // namespace gvdr

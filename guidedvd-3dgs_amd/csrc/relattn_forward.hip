@@ -1,0 +1,661 @@
+// relattn_forward.hip -- attention with a learned relative position bias, forward, for gfx950 (C-ABI: include/gvd_relattn.h).
+//
+//     s_ij = scale q_i . k_j + T[bucket(j - pos_i), h],  p = softmax over the keys seen,  o_i = sum_j p_ij v_j
+//
+// The bias is never laid out as [queries, keys]: buckets depend on the distance alone, so a workgroup expands its head's column of the table to one
+// value a distance in LDS (a few hundred floats), and the products' ACCUMULATORS start from bias / scale instead of from zero: the scores leave
+// the matrix unit with the bias in them.  A block of keys that lies entirely further than the last bucket's border starts from one constant.
+//
+//   k_rel_fwd     a wave = 32 or 64 queries, tiles of 64 keys through LDS, online softmax; optionally a part of the keys only (few rows: parts are
+//                 joined by k_rel_join)
+//   k_rel_short   up to 32 queries and keys (the frames of a pixel): a wave walks (batch, head) items, one pass over memory, no barriers
+//   k_rel_few     up to 4 queries against many keys (new tokens against a cache): 8 lanes a key on the vector unit, bound by reading K and V once
+#include <stdlib.h>
+
+#include "relattn_common.h"
+
+namespace gvdd {
+thread_local std::string g_err;
+int fail(int code, const char* what, hipError_t e)
+{
+    char buf[384];
+    if (e != hipSuccess) snprintf(buf, sizeof buf, "%s: %s", what, hipGetErrorString(e));
+    else snprintf(buf, sizeof buf, "%s", what);
+    g_err = buf;
+    return code;
+}
+}  // namespace gvdd
+
+using namespace gvdr;
+
+namespace gvdr {
+
+int compute_units()
+{
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+    return cus;
+}
+
+int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who)
+{
+    auto bad = [&](const char* what) {
+        char buf[256];
+        snprintf(buf, sizeof buf, "%s: %s", who, what);
+        return fail(-1, buf);
+    };
+    if (!p) return bad("no problem given");
+    if (p->B <= 0 || p->H <= 0 || p->Nq <= 0 || p->Nk <= 0) return bad("sizes must be positive");
+    if ((long long)p->B * p->H > 0x7fffffffLL || p->Nq > (1 << 24) || p->Nk > (1 << 24)) return bad("too many (batch, head) items or rows");
+    if ((long long)p->B * p->H * p->Nq > (1LL << 28)) return bad("too many rows of queries");
+    if (p->D != 64) return bad("head dim must be 64");
+    if (p->is_bf16 < 0 || p->is_bf16 > 1 || p->table_type < 0 || p->table_type > 2) return bad("unknown element type");
+    if (p->buckets <= 0 || (p->both && p->buckets % 2)) return bad("buckets must be positive, and even where both directions have their own");
+    const int side = p->both ? p->buckets / 2 : p->buckets;
+    if (side > GVD_RELATTN_MAX_SIDE) return bad("too many buckets");
+    if (!p->first || p->first[0] != 0) return bad("first[0] must be 0");
+    for (int k = 1; k < side; k++)
+        if (p->first[k] < p->first[k - 1]) return bad("first must not descend");
+    if (p->first[side - 1] > GVD_RELATTN_MAX_REACH) return bad("the last bucket begins too far away");
+    if (!(p->scale > 0.f) || !(p->scale < 1e30f) || !(p->scale > 1e-30f)) return bad("scale must be positive and within 1e-30 .. 1e30");
+    if (p->q_start < -(1 << 29) || p->q_start > (1 << 29)) return bad("q_start is out of range");
+    if ((p->q_bs | p->q_rs | p->kv_bs | p->kv_rs | p->o_bs | p->o_rs) & 7) return bad("strides must be multiples of 8 elements");
+    g.H = p->H; g.Nq = p->Nq; g.Nk = p->Nk; g.buckets = p->buckets; g.side = side; g.both = p->both ? 1 : 0; g.causal = p->causal ? 1 : 0;
+    g.reach = p->first[side - 1] > 1 ? p->first[side - 1] : 1;
+    g.q_start = p->q_start; g.table_type = p->table_type;
+    g.scale = p->scale; g.c = p->scale * LOG2E; g.inv_scale = 1.0f / p->scale;
+    g.q_starts = p->q_starts; g.kv_lens = p->kv_lens; g.table = nullptr;
+    g.q_bs = p->q_bs; g.q_rs = p->q_rs; g.kv_bs = p->kv_bs; g.kv_rs = p->kv_rs; g.o_bs = p->o_bs; g.o_rs = p->o_rs;
+    for (int k = 0; k < GVD_RELATTN_MAX_SIDE; k++) g.first[k] = k < side ? p->first[k] : 0x7fffffff;
+    return 0;
+}
+
+}  // namespace gvdr
+
+namespace {
+
+// ---- general rows ------------------------------------------------------------------------------------------------------------
+template <typename T, int QB, bool PART>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
+          float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
+{
+    typedef typename Tr<T>::vec8 vec8;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    __shared__ __attribute__((aligned(16))) T sKb[2][KV_TILE][LDS_ROW];
+    __shared__ __attribute__((aligned(16))) T sVtb[2][64][LDS_ROW];
+    extern __shared__ __attribute__((aligned(16))) float sBias[];
+
+    int bh, tile_y;
+    xcd_item_tile(bh, tile_y);
+    const int qtile = PART ? tile_y / parts : tile_y, part = PART ? tile_y - qtile * parts : 0;
+    const int b = bh / g.H, h = bh - b * g.H;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+    const int start = start_of(g, b), len = len_of(g, b);
+    const T* qb = q + (size_t)b * g.q_bs + (size_t)h * 64;
+    const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64;
+    const T* vb = v + (size_t)b * g.kv_bs + (size_t)h * 64;
+    const int q0 = qtile * (128 * QB), q_last = (q0 + 128 * QB < g.Nq ? q0 + 128 * QB : g.Nq) - 1;
+    // keys [k_lo, k_hi) are walked; those below k_full are seen by every row of the workgroup
+    int k_lo = 0, k_hi = g.causal ? clamp_int(start + q_last + 1, 0, len) : len;
+    const int k_full = g.causal ? clamp_int(start + q0 + 1, 0, len) : len;
+    if (PART) {
+        const int per = ((k_hi + KV_TILE - 1) / KV_TILE + parts - 1) / parts * KV_TILE;
+        k_lo = part * per < k_hi ? part * per : k_hi;
+        k_hi = k_lo + per < k_hi ? k_lo + per : k_hi;
+    }
+
+    int query[QB];
+    vec8 qf[QB][4];
+    f16v o0[QB], o1[QB];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int qi = 0; qi < QB; qi++) {
+        query[qi] = q0 + (wave * QB + qi) * 32 + col;
+        const T* qr = qb + (size_t)(query[qi] < g.Nq ? query[qi] : g.Nq - 1) * (size_t)g.q_rs + 8 * hi;   // (rows past the end: the last one again, not stored)
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) qf[qi][ks] = *reinterpret_cast<const vec8*>(qr + 16 * ks);
+        o0[qi] = f16v{};
+        o1[qi] = f16v{};
+        m[qi] = LOWEST;
+        l[qi] = 0.f;
+    }
+
+    // K and V tiles, two passes of 256 lanes: K rows as they are; V transposed, the two keys of a channel packed into a dword.  Rows at or behind `len`
+    // are zeros (whatever lies there, also NaN, meets a weight of 0); loads are unconditional (the last row again) and issued a tile ahead.
+    vec8 rk[2], rv0, rv1;
+    const int vkp = tid & 31, vc8 = (tid >> 5) * 8;
+    auto prefetch = [&](int kt) {
+#pragma unroll
+        for (int ps = 0; ps < 2; ps++) {
+            const int c = tid + ps * 256, key = kt + (c >> 3);
+            rk[ps] = *reinterpret_cast<const vec8*>(kb + (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + (c & 7) * 8);
+        }
+        const int key = kt + 2 * vkp;
+        rv0 = *reinterpret_cast<const vec8*>(vb + (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + vc8);
+        rv1 = *reinterpret_cast<const vec8*>(vb + (size_t)(key + 1 < len ? key + 1 : len - 1) * (size_t)g.kv_rs + vc8);
+    };
+    auto commit = [&](int kt, int buf) {
+#pragma unroll
+        for (int ps = 0; ps < 2; ps++) {
+            const int c = tid + ps * 256, row = c >> 3;
+            *reinterpret_cast<vec8*>(&sKb[buf][row][(c & 7) * 8]) = kt + row < len ? rk[ps] : vec8{};
+        }
+        const int key = kt + 2 * vkp;
+        const vec8 x0 = key < len ? rv0 : vec8{}, x1 = key + 1 < len ? rv1 : vec8{};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const T2 pr = { x0[i], x1[i] };
+            *reinterpret_cast<T2*>(&sVtb[buf][vc8 + i][2 * vkp]) = pr;
+        }
+    };
+    if (k_lo < k_hi) prefetch(k_lo);
+    fill_bias(g, h, sBias, tid, 256);
+    float far_past = 0.f, far_ahead = 0.f;
+
+    auto tile = [&](int kt, int buf, auto masked_tag) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        if (kt + KV_TILE < k_hi) {
+            commit(kt + KV_TILE, buf ^ 1);
+            if (kt + 2 * KV_TILE < k_hi) prefetch(kt + 2 * KV_TILE);
+        }
+        const T (*sK)[LDS_ROW] = sKb[buf];
+        const T (*sVt)[LDS_ROW] = sVtb[buf];
+        f16v s0[QB], s1[QB];
+        auto scores = [&]() {
+#pragma unroll
+            for (int qi = 0; qi < QB; qi++) {
+                const int first = start + q0 + (wave * QB + qi) * 32;   // position of the block's first query (uniform)
+                if (kt + 63 - first <= -g.reach || kt - first - 31 >= g.reach) {
+                    const float x = kt < first ? far_past : far_ahead;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) { s0[qi][r] = x; s1[qi][r] = x; }
+                } else {
+                    const float* e = sBias + (kt + 4 * hi - first - col + g.reach + PAD);
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        s0[qi][r] = e[(r & 3) + 8 * (r >> 2)];
+                        s1[qi][r] = e[(r & 3) + 8 * (r >> 2) + 32];
+                    }
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                const vec8 a0 = *reinterpret_cast<const vec8*>(&sK[col][16 * ks + 8 * hi]);
+                const vec8 a1 = *reinterpret_cast<const vec8*>(&sK[32 + col][16 * ks + 8 * hi]);
+#pragma unroll
+                for (int qi = 0; qi < QB; qi++) {
+                    s0[qi] = Tr<T>::mfma(a0, qf[qi][ks], s0[qi]);
+                    s1[qi] = Tr<T>::mfma(a1, qf[qi][ks], s1[qi]);
+                }
+            }
+            if (MASKED) {
+#pragma unroll
+                for (int qi = 0; qi < QB; qi++) {
+                    const int seen = (g.causal && start + query[qi] + 1 < len ? start + query[qi] + 1 : len) - kt - 4 * hi;
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int row = (r & 3) + 8 * (r >> 2);
+                        if (row >= seen) s0[qi][r] = -INFINITY;
+                        if (row + 32 >= seen) s1[qi][r] = -INFINITY;
+                    }
+                }
+            }
+        };
+        scores();
+        unsigned pk0[QB][8], pk1[QB][8];
+#pragma unroll
+        for (int qi = 0; qi < QB; qi++) {
+            float mt = fmaxf(s0[qi][0], s1[qi][0]);
+#pragma unroll
+            for (int r = 1; r < 16; r++) mt = max3f(mt, s0[qi][r], s1[qi][r]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const float m_new = fmaxf(m[qi], mt * g.c);
+            const float alpha = __builtin_amdgcn_exp2f(m[qi] - m_new);
+            m[qi] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j], g.c, -m_new)), p1 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j + 1], g.c, -m_new));
+                const float p2 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j], g.c, -m_new)), p3 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j + 1], g.c, -m_new));
+                pk0[qi][j] = Tr<T>::pack2(p0, p1);
+                pk1[qi][j] = Tr<T>::pack2(p2, p3);
+                sum += (p0 + p1) + (p2 + p3);
+            }
+            l[qi] = fmaf(l[qi], alpha, sum + __shfl_xor(sum, 32, 64));
+#pragma unroll
+            for (int r = 0; r < 16; r++) { o0[qi][r] *= alpha; o1[qi][r] *= alpha; }
+        }
+#pragma unroll
+        for (int kbk = 0; kbk < 2; kbk++)
+#pragma unroll
+            for (int k2 = 0; k2 < 2; k2++) {
+                const int kcol = 32 * kbk + 16 * k2 + 8 * hi;
+                const vec8 a0 = *reinterpret_cast<const vec8*>(&sVt[col][kcol]);
+                const vec8 a1 = *reinterpret_cast<const vec8*>(&sVt[32 + col][kcol]);
+#pragma unroll
+                for (int qi = 0; qi < QB; qi++) {
+                    const vec8 pf = packed_c_to_b_operand<T>(kbk == 0 ? pk0[qi] : pk1[qi], k2);
+                    o0[qi] = Tr<T>::mfma(a0, pf, o0[qi]);
+                    o1[qi] = Tr<T>::mfma(a1, pf, o1[qi]);
+                }
+            }
+        __syncthreads();
+    };
+
+    if (k_lo < k_hi) {   // (uniform over the workgroup)
+        commit(k_lo, 0);
+        if (k_lo + KV_TILE < k_hi) prefetch(k_lo + KV_TILE);
+        __syncthreads();
+        far_past = sBias[0];
+        far_ahead = sBias[bias_len(g.reach) - 1];
+        int kt = k_lo, buf = 0;
+        for (; kt < k_hi && kt + KV_TILE <= k_full; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::false_type{});
+        for (; kt < k_hi; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::true_type{});
+    }
+#pragma unroll
+    for (int qi = 0; qi < QB; qi++) {
+        if (query[qi] >= g.Nq) continue;
+        if (PART) {
+            const size_t row = ((size_t)part * (gridDim.x) + bh) * g.Nq + query[qi];
+            if (hi == 0) part_ml[row] = make_float2(m[qi], l[qi]);
+            float* po = part_o + row * 64;
+#pragma unroll
+            for (int rg = 0; rg < 4; rg++) {
+                const int d0 = 8 * rg + 4 * hi;
+                *reinterpret_cast<float4*>(po + d0) = make_float4(o0[qi][4 * rg], o0[qi][4 * rg + 1], o0[qi][4 * rg + 2], o0[qi][4 * rg + 3]);
+                *reinterpret_cast<float4*>(po + 32 + d0) = make_float4(o1[qi][4 * rg], o1[qi][4 * rg + 1], o1[qi][4 * rg + 2], o1[qi][4 * rg + 3]);
+            }
+            continue;
+        }
+        if (lse && hi == 0) lse[(size_t)bh * g.Nq + query[qi]] = l[qi] > 0.f ? m[qi] + __builtin_amdgcn_logf(l[qi]) : INFINITY;
+        const float inv = l[qi] > 0.f ? 1.0f / l[qi] : 0.f;   // a row that sees nothing: zeros
+        T* orow = out + (size_t)b * g.o_bs + (size_t)h * 64 + (size_t)query[qi] * (size_t)g.o_rs;
+#pragma unroll
+        for (int rg = 0; rg < 4; rg++) {
+            const int d0 = 8 * rg + 4 * hi;
+            uint2 w0, w1;
+            w0.x = Tr<T>::pack2(o0[qi][4 * rg] * inv, o0[qi][4 * rg + 1] * inv);
+            w0.y = Tr<T>::pack2(o0[qi][4 * rg + 2] * inv, o0[qi][4 * rg + 3] * inv);
+            w1.x = Tr<T>::pack2(o1[qi][4 * rg] * inv, o1[qi][4 * rg + 1] * inv);
+            w1.y = Tr<T>::pack2(o1[qi][4 * rg + 2] * inv, o1[qi][4 * rg + 3] * inv);
+            *reinterpret_cast<uint2*>(orow + d0) = w0;
+            *reinterpret_cast<uint2*>(orow + 32 + d0) = w1;
+        }
+    }
+}
+
+// Joins the parts of a row: 16 lanes a row, 4 channels each.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __restrict__ part_o, const float2* __restrict__ part_ml, int parts, int BH,
+                                                  T* __restrict__ out, float* __restrict__ lse)
+{
+    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long long)BH * g.Nq;
+    if (row >= rows) return;
+    const int d0 = (threadIdx.x & 15) * 4;
+    float top = LOWEST;
+    for (int s = 0; s < parts; s++) top = fmaxf(top, part_ml[(size_t)s * rows + row].x);
+    float total = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < parts; s++) {
+        const float2 ml = part_ml[(size_t)s * rows + row];
+        const float w = __builtin_amdgcn_exp2f(ml.x - top);
+        const float4 x = *reinterpret_cast<const float4*>(part_o + ((size_t)s * rows + row) * 64 + d0);
+        total = fmaf(w, ml.y, total);
+        o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    }
+    const long long bh = row / g.Nq;
+    const int n = (int)(row - bh * g.Nq), b = (int)(bh / g.H), h = (int)(bh - (long long)b * g.H);
+    const float inv = total > 0.f ? 1.0f / total : 0.f;
+    uint2 w;
+    w.x = Tr<T>::pack2(o.x * inv, o.y * inv);
+    w.y = Tr<T>::pack2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(out + (size_t)b * g.o_bs + (size_t)n * g.o_rs + (size_t)h * 64 + d0) = w;
+    if (lse && d0 == 0) lse[row] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+}
+
+// ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
+// The whole problem of an item is 3 x 32 x 128 bytes in and 32 x 128 out: memory.  A wave keeps one head (its stride over items is a multiple of H),
+// so its 16 biases a lane stay in registers over all its items; the next item's rows are requested before this one's softmax.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
+                                                   float* __restrict__ lse, int items, int waves)
+{
+    typedef typename Tr<T>::vec8 vec8;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    constexpr int VT_PITCH = 40, O_PITCH = 72;
+    __shared__ __attribute__((aligned(16))) T sVt[4][64][VT_PITCH];
+    __shared__ __attribute__((aligned(16))) T sO[4][32][O_PITCH];
+    __shared__ float sB[4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, r32 = lane & 31;
+    const int gw = blockIdx.x * 4 + wave;
+    if (gw >= waves) return;   // (no barriers below)
+    const int h = gw % g.H, step = waves / g.H, nb = items / g.H;
+    const int kp = lane & 15, vo = lane >> 4;
+    const size_t qoff = (size_t)(r32 < g.Nq ? r32 : g.Nq - 1) * (size_t)g.q_rs + (size_t)h * 64 + 8 * hi;
+    vec8 qf[4], kf[4], va[2], vb[2];
+    int len = 0, len_next;
+    // rows at or behind the length: the last one again; their scores are masked.  (A length of zero: row 0, and the item's result is zeros.)
+    auto load = [&](int b) {
+        len_next = len_of(g, b);
+        const int last = len_next > 0 ? len_next - 1 : 0;
+        const T* qb = q + (size_t)b * g.q_bs + qoff;
+        const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64 + (size_t)(r32 < last ? r32 : last) * (size_t)g.kv_rs + 8 * hi;
+        const T* v0 = v + (size_t)b * g.kv_bs + (size_t)h * 64 + 8 * vo;
+        const size_t off0 = (size_t)(2 * kp < last ? 2 * kp : last) * (size_t)g.kv_rs, off1 = (size_t)(2 * kp + 1 < last ? 2 * kp + 1 : last) * (size_t)g.kv_rs;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            qf[ks] = *reinterpret_cast<const vec8*>(qb + 16 * ks);
+            kf[ks] = *reinterpret_cast<const vec8*>(kb + 16 * ks);
+        }
+#pragma unroll
+        for (int ps = 0; ps < 2; ps++) {
+            va[ps] = *reinterpret_cast<const vec8*>(v0 + off0 + 32 * ps);
+            vb[ps] = *reinterpret_cast<const vec8*>(v0 + off1 + 32 * ps);
+        }
+    };
+    f16v bias;
+    int biased = 0x7fffffff;   // the start that `bias` is for
+    auto set_bias = [&](int start) {
+        sB[wave][lane] = start_value(g, table_at(g, bucket_of(g, lane - 32 - start), h));   // distances -32 .. 31 less the start
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 16; r++) bias[r] = sB[wave][(r & 3) + 8 * (r >> 2) + 4 * hi - r32 + 32];
+        __builtin_amdgcn_wave_barrier();
+        biased = start;
+    };
+    load(gw / g.H);
+    for (int b = gw / g.H; b < nb; b += step) {
+        len = len_next;
+        const int start = start_of(g, b);
+        if (start != biased) set_bias(start);
+#pragma unroll
+        for (int ps = 0; ps < 2; ps++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const T2 pr = { va[ps][i], vb[ps][i] };
+                *reinterpret_cast<T2*>(&sVt[wave][(vo + 4 * ps) * 8 + i][2 * kp]) = pr;
+            }
+        __builtin_amdgcn_wave_barrier();
+        f16v s = bias;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) s = Tr<T>::mfma(kf[ks], qf[ks], s);
+        load(b + step < nb ? b + step : b);
+        const int seen = (g.causal && start + r32 + 1 < len ? start + r32 + 1 : len) - 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
+        float mt = LOWEST;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) mt = max3f(mt, s[r] * g.c, s[r + 1] * g.c);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        unsigned pk[8];
+        float l = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, -mt)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, -mt));
+            pk[j] = Tr<T>::pack2(p0, p1);
+            l += p0 + p1;
+        }
+        l += __shfl_xor(l, 32, 64);
+        f16v o0 = {}, o1 = {};
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            const vec8 pf = packed_c_to_b_operand<T>(pk, k2);
+            const vec8 a0 = *reinterpret_cast<const vec8*>(&sVt[wave][r32][16 * k2 + 8 * hi]);
+            const vec8 a1 = *reinterpret_cast<const vec8*>(&sVt[wave][32 + r32][16 * k2 + 8 * hi]);
+            o0 = Tr<T>::mfma(a0, pf, o0);
+            o1 = Tr<T>::mfma(a1, pf, o1);
+        }
+        const bool empty = !(l > 0.f) || len == 0;   // (a length of zero: row 0 of V was loaded, whatever it holds)
+        if (lse && hi == 0 && r32 < g.Nq) lse[((size_t)b * g.H + h) * g.Nq + r32] = empty ? INFINITY : mt + __builtin_amdgcn_logf(l);
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int rg = 0; rg < 4; rg++) {
+            const int d0 = 8 * rg + 4 * hi;
+            uint2 w0, w1;
+            w0.x = Tr<T>::pack2(o0[4 * rg] * inv, o0[4 * rg + 1] * inv);
+            w0.y = Tr<T>::pack2(o0[4 * rg + 2] * inv, o0[4 * rg + 3] * inv);
+            w1.x = Tr<T>::pack2(o1[4 * rg] * inv, o1[4 * rg + 1] * inv);
+            w1.y = Tr<T>::pack2(o1[4 * rg + 2] * inv, o1[4 * rg + 3] * inv);
+            if (empty) { w0 = make_uint2(0, 0); w1 = make_uint2(0, 0); }
+            *reinterpret_cast<uint2*>(&sO[wave][r32][d0]) = w0;
+            *reinterpret_cast<uint2*>(&sO[wave][r32][32 + d0]) = w1;
+        }
+        __builtin_amdgcn_wave_barrier();
+        T* ob = out + (size_t)b * g.o_bs + (size_t)h * 64 + 8 * (lane & 7);
+#pragma unroll
+        for (int ps = 0; ps < 4; ps++) {
+            const int row = (lane >> 3) + 8 * ps;
+            const uint4 w = *reinterpret_cast<const uint4*>(&sO[wave][row][8 * (lane & 7)]);
+            if (row < g.Nq) *reinterpret_cast<uint4*>(ob + (size_t)row * (size_t)g.o_rs) = w;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- few queries, many keys ----------------------------------------------------------------------------------------------------
+// 8 lanes hold a key's 64 channels, a wave 8 keys at once, 4 of those in flight; every lane group keeps its own running maximum and sum, joined at the end.
+template <typename T, int NQ>
+__global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
+                                                 float* __restrict__ lse, float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
+{
+    typedef typename Tr<T>::vec8 vec8;
+    constexpr int U = 4;
+    __shared__ float sO[4][NQ][64];
+    __shared__ float sM[4][NQ], sL[4][NQ];
+    extern __shared__ __attribute__((aligned(16))) float sBias[];
+    int bh, part;
+    xcd_item_tile(bh, part);
+    const int b = bh / g.H, h = bh - b * g.H;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 3, sub = lane & 7;
+    const int start = start_of(g, b), len = len_of(g, b);
+    const int k_end = g.causal ? clamp_int(start + g.Nq, 0, len) : len;
+    const int per = ((k_end + 127) / 128 + parts - 1) / parts * 128;
+    const int k_lo = part * per < k_end ? part * per : k_end, k_hi = k_lo + per < k_end ? k_lo + per : k_end;
+    const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64 + 8 * sub;
+    const T* vb = v + (size_t)b * g.kv_bs + (size_t)h * 64 + 8 * sub;
+    vec8 kf[U], vf[U];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = base + 8 * u + grp;
+            const size_t off = (size_t)(j < k_hi ? j : k_hi - 1) * (size_t)g.kv_rs;
+            kf[u] = *reinterpret_cast<const vec8*>(kb + off);
+            vf[u] = *reinterpret_cast<const vec8*>(vb + off);
+        }
+    };
+    const int base0 = k_lo + wave * 32;
+    if (base0 < k_hi) load(base0);
+    float qv[NQ][8], acc[NQ][8], m[NQ], l[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const vec8 x = *reinterpret_cast<const vec8*>(q + (size_t)b * g.q_bs + (size_t)(i < g.Nq ? i : g.Nq - 1) * (size_t)g.q_rs + (size_t)h * 64 + 8 * sub);
+#pragma unroll
+        for (int e = 0; e < 8; e++) { qv[i][e] = (float)x[e]; acc[i][e] = 0.f; }
+        m[i] = LOWEST;
+        l[i] = 0.f;
+    }
+    fill_bias(g, h, sBias, tid, 256);
+    __syncthreads();
+    const int span = g.reach + PAD;
+    for (int base = base0; base < k_hi; base += 128) {
+        float kk[U][8], vv[U][8];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) { kk[u][e] = (float)kf[u][e]; vv[u][e] = (float)vf[u][e]; }
+        if (base + 128 < k_hi) load(base + 128);
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            float s[U], top = m[i];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float x = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) x = fmaf(qv[i][e], kk[u][e], x);
+                x += __shfl_xor(x, 1, 64);
+                x += __shfl_xor(x, 2, 64);
+                x += __shfl_xor(x, 4, 64);
+                const int j = base + 8 * u + grp, d = j - start - i;
+                x = (x + sBias[clamp_int(d, -span, span) + span]) * g.c;
+                s[u] = j < k_hi && !(g.causal && d > 0) ? x : -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float alpha = __builtin_amdgcn_exp2f(m[i] - top);
+            m[i] = top;
+            l[i] *= alpha;
+            float p[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) { p[u] = __builtin_amdgcn_exp2f(s[u] - top); l[i] += p[u]; }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float a = acc[i][e] * alpha;
+#pragma unroll
+                for (int u = 0; u < U; u++) a = fmaf(p[u], vv[u][e], a);
+                acc[i][e] = a;
+            }
+        }
+    }
+    // join the wave's 8 lane groups, then the workgroup's 4 waves
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        float top = m[i];
+#pragma unroll
+        for (int x = 8; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        const float w = __builtin_amdgcn_exp2f(m[i] - top);
+        float sum = l[i] * w;
+#pragma unroll
+        for (int x = 8; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float a = acc[i][e] * w;
+#pragma unroll
+            for (int x = 8; x < 64; x <<= 1) a += __shfl_xor(a, x, 64);
+            if (grp == 0) sO[wave][i][8 * sub + e] = a;
+        }
+        if (lane == 0) { sM[wave][i] = top; sL[wave][i] = sum; }
+    }
+    __syncthreads();
+    for (int t = tid; t < NQ * 64; t += 256) {
+        const int i = t >> 6, d = t & 63;
+        if (i >= g.Nq) continue;
+        const float top = fmaxf(fmaxf(sM[0][i], sM[1][i]), fmaxf(sM[2][i], sM[3][i]));
+        float total = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(sM[w][i] - top);
+            total = fmaf(f, sL[w][i], total);
+            o = fmaf(f, sO[w][i][d], o);
+        }
+        if (parts > 1) {
+            const size_t row = ((size_t)part * gridDim.x + bh) * g.Nq + i;
+            part_o[row * 64 + d] = o;
+            if (d == 0) part_ml[row] = make_float2(top, total);
+        } else {
+            out[(size_t)b * g.o_bs + (size_t)i * g.o_rs + (size_t)h * 64 + d] = (T)(total > 0.f ? o / total : 0.f);
+            if (lse && d == 0) lse[(size_t)bh * g.Nq + i] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+enum Form { SHORT, FEW, GENERAL };
+
+struct Plan { Form form; int qb, tiles, parts; };
+
+// Which kernel, and into how many parts the keys are cut.
+Plan plan_of(const Geo& g, int B, int cus)
+{
+    const long long bh = (long long)B * g.H;
+    if (g.Nq <= 32 && g.Nk <= 32) return { SHORT, 1, 1, 1 };
+    Plan pl;
+    pl.form = g.Nq <= 4 ? FEW : GENERAL;
+    pl.qb = pl.form == GENERAL && g.Nq >= 512 ? 2 : 1;
+    pl.tiles = pl.form == FEW ? 1 : (g.Nq + 128 * pl.qb - 1) / (128 * pl.qb);
+    const long long wgs = bh * pl.tiles, want = (long long)cus * (pl.form == FEW ? 8 : 2);
+    const int least = pl.form == FEW ? 256 : 512;   // keys a part
+    long long parts = wgs < want ? (want + wgs - 1) / wgs : 1;
+    const long long most = (g.Nk + least - 1) / least;
+    if (parts > most) parts = most;
+    if (parts > 64) parts = 64;
+    pl.parts = (int)parts;
+    return pl;
+}
+
+size_t part_rows(const Geo& g, int B, const Plan& pl) { return (size_t)pl.parts * B * g.H * g.Nq; }
+
+template <typename T>
+int launch_fwd(const Geo& g, int B, const void* q, const void* k, const void* v, void* out, float* lse, void* ws, hipStream_t stream)
+{
+    const int cus = compute_units();
+    const Plan pl = plan_of(g, B, cus);
+    const int BH = B * g.H;
+    if (pl.form != SHORT && (BH > (1 << 23) || (long long)pl.tiles * pl.parts > 65535)) return fail(-1, "gvd_relattn_fwd: too many workgroups");
+    float* po = nullptr;
+    float2* ml = nullptr;
+    if (pl.parts > 1) {
+        if (!ws) return fail(-1, "gvd_relattn_fwd: this problem needs a workspace");
+        if ((uintptr_t)ws & 15) return fail(-1, "gvd_relattn_fwd: the workspace must be 16-byte aligned");
+        po = (float*)ws;
+        ml = (float2*)(po + part_rows(g, B, pl) * 64);
+    }
+    const size_t lds = sizeof(float) * bias_len(g.reach);
+    if (pl.form == SHORT) {
+        // as many waves as stay resident (4 workgroups a CU by LDS), a multiple of the heads
+        long long waves = (long long)cus * 16;
+        if (waves > BH) waves = BH;
+        waves = waves >= g.H ? waves / g.H * g.H : g.H;
+        hipLaunchKernelGGL(k_rel_short<T>, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, BH, (int)waves);
+    } else if (pl.form == FEW) {
+        const dim3 grid((unsigned)BH, (unsigned)pl.parts);
+#define GVD_FEW(N) hipLaunchKernelGGL((k_rel_few<T, N>), grid, dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
+        if (g.Nq == 1) GVD_FEW(1); else if (g.Nq == 2) GVD_FEW(2); else GVD_FEW(4);
+#undef GVD_FEW
+    } else {
+        const dim3 grid((unsigned)BH, (unsigned)(pl.tiles * pl.parts));
+#define GVD_GEN(Q, P) hipLaunchKernelGGL((k_rel_fwd<T, Q, P>), grid, dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
+        if (pl.qb == 2) { if (pl.parts > 1) GVD_GEN(2, true); else GVD_GEN(2, false); }
+        else            { if (pl.parts > 1) GVD_GEN(1, true); else GVD_GEN(1, false); }
+#undef GVD_GEN
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(-2, "launch k_rel_*", e);
+    if (pl.parts > 1) {
+        const long long rows = (long long)BH * g.Nq;
+        hipLaunchKernelGGL(k_rel_join<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, g, po, ml, pl.parts, BH, (T*)out, lse);
+        e = hipGetLastError();
+        if (e != hipSuccess) return fail(-2, "launch k_rel_join", e);
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* gvd_relattn_last_error(void) { return gvdd::g_err.c_str(); }
+
+long long gvd_relattn_fwd_workspace(const gvd_relattn_problem* p)
+{
+    Geo g;
+    const int rc = make_geo(p, g, "gvd_relattn_fwd_workspace");
+    if (rc) return rc;
+    const Plan pl = plan_of(g, p->B, compute_units());
+    return pl.parts > 1 ? (long long)(part_rows(g, p->B, pl) * (64 * sizeof(float) + sizeof(float2))) : 0;
+}
+
+int gvd_relattn_fwd(const gvd_relattn_problem* p, const void* q, const void* k, const void* v, const void* table, void* out, float* lse,
+                    void* workspace, void* stream)
+{
+    Geo g;
+    const int rc = make_geo(p, g, "gvd_relattn_fwd");
+    if (rc) return rc;
+    if (!q || !k || !v || !table || !out) return fail(-1, "gvd_relattn_fwd: null pointer");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) return fail(-1, "gvd_relattn_fwd: pointers must be 16-byte aligned");
+    g.table = table;
+    return p->is_bf16 ? launch_fwd<__bf16>(g, p->B, q, k, v, out, lse, workspace, (hipStream_t)stream)
+                      : launch_fwd<_Float16>(g, p->B, q, k, v, out, lse, workspace, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -6,6 +6,7 @@ fallback: CPU tensors raise unless a test has explicitly enabled the reference m
 `use_reference_math(True)` (the `-m "not gpu"` tests of the host logic / module structure do that).
 
     attention(q, k, v, heads)          softmax(q k^T / sqrt(d)) v per head, q [B,Nq,h*d], k/v [B,Nk,h*d]
+    relative_bias_attention(q, k, v, table, heads)   the same with a learned bias by buckets of relative position (csrc/relattn_*.hip)
     group_norm(x, groups, w, b, eps, silu)   fp32 statistics (lvdm/basics.py:76-78), optional fused SiLU
     ddim_step(...)                     the whole no-grad DDIM update of ddim.py:208-280 in one kernel
 """
@@ -407,6 +408,24 @@ def attention(q, k, v, heads, frame_major=False, accum=None, accum_scale=1.0):
         v = v.expand(*[q.shape[bd] if i == bd else -1 for i in range(3)])
     o = attention_math(q, k, v, heads, frame_major)
     return o if accum is None else accum + accum_scale * o
+
+
+def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirectional=True, causal=False, q_start=0, kv_lens=None, scale=None,
+                            frame_major=False):
+    """Attention with a learned bias by relative position: softmax_j(scale q_i . k_j + table[bucket(j - (q_start + i)), h]) v_j per head.
+
+    q [B, Nq, h*64], k / v [B, Nk, h*64] (or [1, Nk, h*64]: shared by the batch); frame_major: [N, B, h*64], as in `attention`.  fp16 or bf16.
+    table [buckets, heads], float32, fp16 or bf16; gradients of q, k, v and table (no atomics across workgroups: the same call gives the same bits).
+    bucket(d): the first half of a side's buckets hold one distance each, the others equal ratios up to max_distance, the last everything beyond;
+        bidirectional: keys ahead (d > 0) have the table's upper half; otherwise they share bucket 0 (`relative.relative_buckets`).
+        An entry at or below -10000 (-infinity, a type's lowest value) masks its bucket; one above 10000 counts as 10000.
+    causal: keys j <= q_start + i only.  q_start: position of query 0 among the keys, a number, or (inference) int32 [B]: new tokens against a cache.
+    kv_lens int32 [B]: keys and values at and behind it are not seen, whatever they hold (their gradients are zeros); 0 is a length.  Rows of k and v before it
+        have to be finite also where causal hides them from some queries.
+    A query that sees nothing gives zeros and has no gradient.  scale: default 64 ** -0.5."""
+    from . import relative
+    return relative.relative_bias_attention(q, k, v, table, heads, max_distance=max_distance, bidirectional=bidirectional, causal=causal, q_start=q_start,
+                                            kv_lens=kv_lens, scale=scale, frame_major=frame_major)
 
 
 # --------------------------------------------------------------------------------------------------
