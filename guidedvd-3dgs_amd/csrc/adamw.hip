@@ -208,7 +208,7 @@ __device__ __forceinline__ float finite_max(f4 x)
     return r;
 }
 
-// A block whose largest magnitude is below this is held as zeros: 448 / big would overflow.  (A root is never that small unless it is 0: the least
+// A block whose largest magnitude is below this is held as zeros: 1 / big would overflow.  (A root is never that small unless it is 0: the least
 // positive float's root is 3.7e-23.)
 constexpr float TINY = 0x1p-110f;
 
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(256) k_adamw8(const Table a, float w1, float b
         }
         store4(p, i, n, wide, pn);
         const float bm = wave_max(finite_max(mn)), br = wave_max(finite_max(rn));   // (elements beyond n: zeros)
-        const float fm = bm >= TINY ? 448.f / bm : 0.f, fr = br >= TINY ? 448.f / br : 0.f;
+        const float fm = bm >= TINY ? 1.f / bm * 448.f : 0.f, fr = br >= TINY ? 1.f / br * 448.f : 0.f;
         unsigned cm = 0, cr = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {

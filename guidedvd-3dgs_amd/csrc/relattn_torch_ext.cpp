@@ -1,0 +1,203 @@
+// relattn_torch_ext.cpp -- relative_bias_attention as one torch::autograd::Function over the C-ABI (include/gvd_relattn.h): checks of arguments, strides, outputs,
+// workspaces, and the backward without Python.  No kernel lives here.  With a Python autograd function a training pass took 180 us of host time, as much
+// as its kernels at the sizes of a temporal layer.
+//
+// Plain C++ (g++); the entry points are resolved from the library path that Python hands to init(), so A/B builds share one instance.
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <dlfcn.h>
+
+#include "../../include/gvd_relattn.h"
+
+namespace {
+
+struct Api {
+    decltype(&gvd_relattn_fwd) fwd = nullptr;
+    decltype(&gvd_relattn_bwd) bwd = nullptr;
+    decltype(&gvd_relattn_fwd_workspace) fwd_workspace = nullptr;
+    decltype(&gvd_relattn_bwd_workspace) bwd_workspace = nullptr;
+    decltype(&gvd_relattn_last_error) last_error = nullptr;
+} g_api;
+
+void init(const std::string& path)
+{
+    void* h = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+    TORCH_CHECK(h != nullptr, "cannot load ", path, ": ", dlerror());
+    auto sym = [&](const char* name) {
+        void* p = dlsym(h, name);
+        TORCH_CHECK(p != nullptr, path, " does not export ", name);
+        return p;
+    };
+    g_api.fwd = reinterpret_cast<decltype(g_api.fwd)>(sym("gvd_relattn_fwd"));
+    g_api.bwd = reinterpret_cast<decltype(g_api.bwd)>(sym("gvd_relattn_bwd"));
+    g_api.fwd_workspace = reinterpret_cast<decltype(g_api.fwd_workspace)>(sym("gvd_relattn_fwd_workspace"));
+    g_api.bwd_workspace = reinterpret_cast<decltype(g_api.bwd_workspace)>(sym("gvd_relattn_bwd_workspace"));
+    g_api.last_error = reinterpret_cast<decltype(g_api.last_error)>(sym("gvd_relattn_last_error"));
+}
+
+long long check(long long rc)
+{
+    TORCH_CHECK(rc >= 0, "gvd_relattn error ", rc, ": ", g_api.last_error());
+    return rc;
+}
+
+struct Config {
+    at::Tensor first, kv_lens;   // CPU int32: the least distance of each bucket of one side; device int32 or undefined
+    int64_t heads, q_start;
+    bool both, causal, frame_major;
+    double scale;
+    int batch_dim() const { return frame_major ? 1 : 0; }
+    int row_dim() const { return frame_major ? 0 : 1; }
+};
+
+bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+at::Tensor packed(const at::Tensor& t)   // contiguous and 16-byte aligned (a contiguous view may begin anywhere)
+{
+    at::Tensor c = t.contiguous();
+    return aligned(c) ? c : c.clone();
+}
+
+bool in_place(const at::Tensor& t) { return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); }
+
+// (batch, row) strides; a batch of one serves any batch, and the stride of a dimension of one row is never used
+std::pair<long long, long long> strides(const at::Tensor& t, const Config& c)
+{
+    const int bd = c.batch_dim(), rd = c.row_dim();
+    return {t.size(bd) == 1 ? 0 : t.stride(bd), t.size(rd) == 1 ? t.size(2) : t.stride(rd)};
+}
+
+gvd_relattn_problem problem(const at::Tensor& q, const at::Tensor& k, const at::Tensor& out, const at::Tensor& table, const at::Tensor& q_starts, const Config& c)
+{
+    gvd_relattn_problem p = {};
+    p.B = (int)q.size(c.batch_dim());
+    p.H = (int)c.heads;
+    p.Nq = (int)q.size(c.row_dim());
+    p.Nk = (int)k.size(c.row_dim());
+    p.D = (int)(q.size(2) / c.heads);
+    p.is_bf16 = q.scalar_type() == at::kBFloat16;
+    p.table_type = table.scalar_type() == at::kFloat ? 0 : table.scalar_type() == at::kHalf ? 1 : 2;
+    p.buckets = (int)table.size(0);
+    p.both = c.both;
+    p.causal = c.causal;
+    p.first = c.first.data_ptr<int>();
+    p.scale = (float)c.scale;
+    p.q_start = (int)c.q_start;
+    p.q_starts = q_starts.defined() ? q_starts.data_ptr<int>() : nullptr;
+    p.kv_lens = c.kv_lens.defined() ? c.kv_lens.data_ptr<int>() : nullptr;
+    std::tie(p.q_bs, p.q_rs) = strides(q, c);
+    std::tie(p.kv_bs, p.kv_rs) = strides(k, c);
+    std::tie(p.o_bs, p.o_rs) = strides(out, c);
+    return p;
+}
+
+at::Tensor bytes(long long n, const at::Tensor& like) { return n ? at::empty({n}, like.options().dtype(at::kByte)) : at::Tensor(); }
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* stream_of(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+at::Tensor forward_(at::Tensor q, at::Tensor k, at::Tensor v, const at::Tensor& table, const at::Tensor& q_starts, const Config& c, at::Tensor* lse)
+{
+    const c10::DeviceGuard guard(q.device());
+    const int bd = c.batch_dim(), rd = c.row_dim();
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    if (lse) *lse = at::empty({q.size(bd), c.heads, q.size(rd)}, q.options().dtype(at::kFloat));
+    if (q.numel() == 0 || k.size(rd) == 0) return out.zero_();
+    if (!in_place(q)) q = packed(q);
+    if (!in_place(k)) k = packed(k);
+    if (!in_place(v)) v = packed(v);
+    if (strides(k, c) != strides(v, c)) {
+        k = packed(k);
+        v = packed(v);
+    }
+    const gvd_relattn_problem p = problem(q, k, out, table, q_starts, c);
+    const at::Tensor ws = bytes(check(g_api.fwd_workspace(&p)), q);
+    check(g_api.fwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr, ptr(ws), stream_of(q)));
+    return out;
+}
+
+struct RelativeBiasAttention : torch::autograd::Function<RelativeBiasAttention> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& table,
+                              const Config& c)
+    {
+        const at::Tensor q = packed(q_), k = packed(k_), v = packed(v_);
+        at::Tensor lse;
+        const at::Tensor out = forward_(q, k, v, table, at::Tensor(), c, &lse);
+        torch::autograd::variable_list saved = {q, k, v, table, out, lse};
+        if (c.kv_lens.defined()) saved.push_back(c.kv_lens);
+        ctx->save_for_backward(saved);
+        ctx->saved_data["first"] = c.first;
+        ctx->saved_data["heads"] = c.heads;
+        ctx->saved_data["q_start"] = c.q_start;
+        ctx->saved_data["flags"] = (int64_t)(c.both | c.causal << 1 | c.frame_major << 2);
+        ctx->saved_data["scale"] = c.scale;
+        return out;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "relative_bias_attention: its gradients have no gradients (create_graph=True)");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out = saved[4], &lse = saved[5];
+        const int64_t flags = ctx->saved_data["flags"].toInt();
+        const Config c = {ctx->saved_data["first"].toTensor(), saved.size() > 6 ? saved[6] : at::Tensor(), ctx->saved_data["heads"].toInt(), ctx->saved_data["q_start"].toInt(), (flags & 1) != 0, (flags & 2) != 0,
+                          (flags & 4) != 0, ctx->saved_data["scale"].toDouble()};
+        const c10::DeviceGuard guard(q.device());
+        at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dtable = at::empty_like(table);
+        if (q.numel() == 0 || k.numel() == 0) {
+            for (at::Tensor* t : {&dq, &dk, &dv, &dtable}) t->zero_();
+        } else {
+            const at::Tensor g = packed(grads[0]);
+            const gvd_relattn_problem p = problem(q, k, out, table, at::Tensor(), c);
+            const at::Tensor ws = bytes(check(g_api.bwd_workspace(&p)), q);
+            check(g_api.bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                            dv.data_ptr(), dtable.data_ptr(), ptr(ws), stream_of(q)));
+        }
+        return {dq, dk, dv, dtable, at::Tensor()};
+    }
+};
+
+#define GVD_WANT(cond, ...) TORCH_CHECK_VALUE(cond, "relative_bias_attention: ", __VA_ARGS__)
+
+// q, k, v: 16-bit, on one device, heads of 64 (the caller has looked).
+at::Tensor attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Tensor& table_, int64_t heads, const at::Tensor& first, bool both, bool causal, int64_t q_start,
+                  const c10::optional<at::Tensor>& q_starts_, const c10::optional<at::Tensor>& kv_lens_, double scale, bool frame_major)
+{
+    const at::Tensor q_starts = q_starts_.value_or(at::Tensor()), kv_lens = kv_lens_.value_or(at::Tensor());
+    const Config c = {first, kv_lens, heads, q_start, both, causal, frame_major, scale};
+    const int bd = c.batch_dim();
+    GVD_WANT(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes(), "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), ": three dimensions each, k and v of one shape");
+    const int64_t B = q.size(bd), C = q.size(2);
+    GVD_WANT(heads > 0 && C % heads == 0 && k.size(2) == C && (k.size(bd) == 1 || k.size(bd) == B), "q ", q.sizes(), ", k ", k.sizes(), " with ", heads,
+             " heads: channels heads * d on either side, and one batch size (or one K / V for the whole batch)");
+    GVD_WANT(table_.dim() == 2 && table_.size(1) == heads && table_.size(0) == (both ? 2 : 1) * first.numel() &&
+                 (table_.scalar_type() == at::kFloat || table_.scalar_type() == at::kHalf || table_.scalar_type() == at::kBFloat16),
+             "table ", table_.scalar_type(), " ", table_.sizes(), ": [buckets, heads] of float32, float16 or bfloat16, an even number of buckets where both directions have "
+             "their own");
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&k, &v, &table_}) GVD_WANT(t->device() == q.device(), t == &k ? "k" : t == &v ? "v" : "table", " is on ", t->device(), ", q on ", q.device());
+    for (const at::Tensor* t : {&q_starts, &kv_lens})
+        GVD_WANT(!t->defined() || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->device() == q.device() && t->is_contiguous()),
+                 t == &kv_lens ? "kv_lens" : "q_start", ": ", t->scalar_type(), " ", t->sizes(), " on ", t->device(), "; a contiguous int32 [", B, "] on ", q.device(), " is wanted");
+    const at::Tensor table = table_.contiguous();
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || table.requires_grad())) {
+        TORCH_CHECK_NOT_IMPLEMENTED(!q_starts.defined(), "relative_bias_attention: gradients with one q_start for the whole batch only (a tensor of them is for inference)");
+        if (k.size(bd) != B) {   // one K / V for the whole batch: the backward addresses one per entry, autograd sums their gradients
+            std::vector<int64_t> shape = k.sizes().vec();
+            shape[bd] = B;
+            k = k.expand(shape);
+            v = v.expand(shape);
+        }
+        return RelativeBiasAttention::apply(q, k, v, table, c);
+    }
+    return forward_(q, k, v, table, q_starts, c, nullptr);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
+{
+    m.doc() = "relative_bias_attention over libgvd_relattn.so (see csrc/relattn_torch_ext.cpp)";
+    m.def("init", &init, "resolve the C-ABI entry points from the given library path");
+    m.def("attend", &attend, "attention with a learned relative position bias, differentiable");
+}

@@ -10,44 +10,17 @@ state_bits=8 the moments take 2 bytes an element instead of 8; `moments` / `set_
 parameters raise.
 """
 import ctypes
+import importlib.util
 import math
 import os
-import struct
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.environ.get("GVD_OPTIM_LIB") or os.path.join(os.path.dirname(_HERE), "lib", "libgvd_optim.so")  # env: A/B builds
-_LIB = None
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_TENSOR = struct.Struct("6Qq3fI")          # gvd_adamw_tensor
+_EXT_PATH = os.path.join(os.path.dirname(_HERE), "lib", "_gvd_optim_torch.so")
+_LIB = _EXT = None
 BLOCK = 256                                 # GVD_ADAMW_BLOCK: elements that share a scale where moments are held in 8 bits
-
-
-class _Noop:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *a):
-        return False
-
-
-_NOOP = _Noop()
-
-
-def _on(dev):
-    """Device guard that is free when `dev` is already the current device (torch.cuda.device() costs ~25 us per use)."""
-    idx = dev.index
-    return _NOOP if idx is None or idx == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _stream():
-    if _RAW_STREAM is not None:
-        return _RAW_STREAM(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
 
 
 def lib():
@@ -60,14 +33,23 @@ def lib():
         L.gvd_optim_last_error.restype = ctypes.c_char_p
         L.gvd_adamw_key.restype = ctypes.c_uint
         L.gvd_adamw_key.argtypes = [ctypes.c_uint] * 3
-        L.gvd_adamw_step.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 3 + [ctypes.c_void_p] * 2
         _LIB = L
     return _LIB
 
 
-def _check(rc):
-    if rc != 0:
-        raise RuntimeError(f"gvd_optim error {rc}: {lib().gvd_optim_last_error().decode()}")
+def ext():
+    """The compiled host half of the step (csrc/optim_torch_ext.cpp) over the same library instance."""
+    global _EXT
+    if _EXT is None:
+        lib()
+        if not os.path.exists(_EXT_PATH):
+            raise RuntimeError(f"{_EXT_PATH} is missing: build the extensions first (python -c 'import __graft_entry__ as g; g.build()')")
+        spec = importlib.util.spec_from_file_location("_gvd_optim_torch", _EXT_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.init(_LIB_PATH)
+        _EXT = mod
+    return _EXT
 
 
 def _dense(t):
@@ -250,79 +232,36 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         launches, place = {}, -1
         for g in self.param_groups:
-            common = None
+            (b1, b2), bits, capturable, lr = g["betas"], g["state_bits"], bool(g["capturable"]), g["lr"]
+            common = (b1, b2, g["eps"], bits, capturable, g["seed"] if bits == 8 else 0)
+            names = ("step", "exp_avg", "exp_avg_sq") if bits == 32 else ("step", "exp_avg", "exp_avg_rms", "exp_avg_scale", "exp_avg_rms_scale")
+            device = dtype = None
             for p in g["params"]:
                 place += 1
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                grad = self._gradient(p)
+                if not p.is_cuda:
+                    raise RuntimeError(f"FusedAdamW: parameter on {p.device}; this build has no CPU path")
                 st = self.state[p]
                 if not st:
                     st.update(self._new_state(p, g))
-                if common is None:
-                    (b1, b2), bits, capturable = g["betas"], g["state_bits"], bool(g["capturable"])
-                    common = (float(b1), float(b2), float(g["eps"]), bits, capturable, g["seed"] if bits == 8 or capturable else 0)
-                self._check_state(p, st, common[3])
-                launches.setdefault((p.device, p.dtype) + common, []).append((p, grad, st, g, place))
-        for (device, dtype, b1, b2, eps, bits, capturable, seed), items in launches.items():
-            with _on(device):
-                if torch.cuda.is_current_stream_capturing() and not capturable:
-                    raise RuntimeError("FusedAdamW: step() in a graph capture needs capturable=True (the count of steps would be frozen)")
-                self._launch(items, device, dtype, b1, b2, eps, bits, capturable, seed)
+                if p.dtype is not dtype or p.device != device:
+                    device, dtype = p.device, p.dtype
+                    flat, lrs, lr_at, decays, places = launches.setdefault((device, dtype) + common, ([], [], [], [], []))
+                flat.append(p)
+                flat.append(grad)
+                try:
+                    flat.extend([st[n] for n in names])
+                except KeyError as e:
+                    raise RuntimeError(f"FusedAdamW: the state {e} of a parameter is missing: it does not fit state_bits={bits}") from None
+                if capturable:
+                    lr_at.append(lr if torch.is_tensor(lr) else None)
+                lrs.append(0.0 if torch.is_tensor(lr) else lr)
+                decays.append(g["weight_decay"])
+                places.append(place)
+        for (device, dtype, b1, b2, eps, bits, capturable, seed), (flat, lrs, lr_at, decays, places) in launches.items():
+            if not capturable and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: step() in a graph capture needs capturable=True (the count of steps would be frozen)")
+            ext().adamw_step(flat, lrs, lr_at, decays, places, b1, b2, eps, bits, capturable, seed)
         return loss
-
-    @staticmethod
-    def _gradient(p):
-        g = p.grad
-        if not p.is_cuda:
-            raise RuntimeError(f"FusedAdamW: parameter on {p.device}; this build has no CPU path")
-        if p.dtype not in _TYPES:
-            raise TypeError(f"FusedAdamW: parameters are float32, float16 or bfloat16, not {p.dtype}")
-        if g.layout != torch.strided:
-            raise RuntimeError("FusedAdamW: sparse gradients are not supported")
-        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-            raise RuntimeError(f"FusedAdamW: a gradient of {g.dtype} {tuple(g.shape)} on {g.device} for a parameter of {p.dtype} {tuple(p.shape)} on {p.device}")
-        if not _dense(p):
-            raise RuntimeError("FusedAdamW: parameters must be dense (no gaps, no element twice)")
-        if g.stride() != p.stride() and p.numel() > 1:
-            g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-        return g
-
-    @staticmethod
-    def _launch(items, device, dtype, b1, b2, eps, bits, capturable, seed):
-        L = lib()
-        ptr = torch.Tensor.data_ptr
-        buf = bytearray(_TENSOR.size * len(items))
-        second = "exp_avg_sq" if bits == 32 else "exp_avg_rms"
-        if len({ptr(it[0]) for it in items if it[0].numel()}) != sum(1 for it in items if it[0].numel()):
-            raise RuntimeError("FusedAdamW: two parameters share their memory")
-        scalars, size, factor, keep, key = None, 0.0, 0.0, 0.0, 0
-        if capturable:
-            n = len(items)
-            scalars = torch.empty(4 * n, dtype=torch.float32, device=device)
-            P = ctypes.c_void_p
-            for _, _, st, g, _ in items:
-                if st["step"].device != device or st["step"].dtype != torch.float32:
-                    raise RuntimeError("FusedAdamW: with capturable=True the state's 'step' is a float32 on the parameter's device")
-                if torch.is_tensor(g["lr"]) and g["lr"].device != device:
-                    raise RuntimeError("FusedAdamW: lr is on another device than its parameters")
-            _check(L.gvd_adamw_scalars((P * n)(*[ptr(it[2]["step"]) for it in items]),
-                                       (P * n)(*[ptr(it[3]["lr"]) if torch.is_tensor(it[3]["lr"]) else None for it in items]),
-                                       (ctypes.c_double * n)(*[0.0 if torch.is_tensor(it[3]["lr"]) else it[3]["lr"] for it in items]),
-                                       (ctypes.c_double * n)(*[it[3]["weight_decay"] for it in items]),
-                                       (ctypes.c_uint * n)(*[it[4] for it in items]), n, ctypes.c_double(b1), ctypes.c_double(b2),
-                                       ctypes.c_uint(seed), P(ptr(scalars)), P(_stream())))
-        at = 0
-        for p, grad, st, g, place in items:
-            if not capturable:
-                t = st["step"]
-                t += 1
-                t = t.item()
-                size, factor = g["lr"] / (1.0 - b1 ** t), 1.0 / math.sqrt(1.0 - b2 ** t)
-                keep = 1.0 - g["lr"] * g["weight_decay"]
-                if bits == 8:
-                    key = L.gvd_adamw_key(seed, place, int(t))
-            _TENSOR.pack_into(buf, at, ptr(p), ptr(grad), ptr(st["exp_avg"]), ptr(st[second]), ptr(st["exp_avg_scale"]) if bits == 8 else 0,
-                              ptr(st["exp_avg_rms_scale"]) if bits == 8 else 0, p.numel(), size, factor, keep, key)
-            at += _TENSOR.size
-        _check(L.gvd_adamw_step(bytes(buf), len(items), _TYPES[dtype], bits, b1, b2, eps, None if scalars is None else ptr(scalars), _stream()))

@@ -3,6 +3,7 @@ C-ABI library lib/libgvd_relattn.so (include/gvd_relattn.h).  The entry point is
 """
 import ctypes
 import functools
+import importlib.util
 import os
 
 import torch
@@ -11,16 +12,10 @@ from . import ops
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.environ.get("GVD_RELATTN_LIB") or os.path.join(os.path.dirname(_HERE), "lib", "libgvd_relattn.so")  # env: A/B builds
-_LIB = None
+_EXT_PATH = os.path.join(os.path.dirname(_HERE), "lib", "_gvd_relattn_torch.so")
+_LIB = _EXT = None
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_SIDE, MAX_DISTANCE = 128, 1024      # GVD_RELATTN_MAX_SIDE, GVD_RELATTN_MAX_REACH
-
-
-class _Problem(ctypes.Structure):       # gvd_relattn_problem
-    _fields_ = ([(n, ctypes.c_int) for n in ("B", "H", "Nq", "Nk", "D", "is_bf16", "table_type", "buckets", "both", "causal")]
-                + [("first", ctypes.POINTER(ctypes.c_int)), ("scale", ctypes.c_float), ("q_start", ctypes.c_int), ("q_starts", ctypes.c_void_p),
-                   ("kv_lens", ctypes.c_void_p)]
-                + [(n, ctypes.c_longlong) for n in ("q_bs", "q_rs", "kv_bs", "kv_rs", "o_bs", "o_rs")])
 
 
 def lib():
@@ -32,17 +27,24 @@ def lib():
         L = ctypes.CDLL(_LIB_PATH)
         L.gvd_relattn_last_error.restype = ctypes.c_char_p
         for f in (L.gvd_relattn_fwd_workspace, L.gvd_relattn_bwd_workspace):
-            f.restype, f.argtypes = ctypes.c_longlong, [ctypes.POINTER(_Problem)]
-        L.gvd_relattn_fwd.argtypes = [ctypes.POINTER(_Problem)] + [ctypes.c_void_p] * 8
-        L.gvd_relattn_bwd.argtypes = [ctypes.POINTER(_Problem)] + [ctypes.c_void_p] * 13
+            f.restype = ctypes.c_longlong
         _LIB = L
     return _LIB
 
 
-def _check(rc):
-    if rc < 0:
-        raise RuntimeError(f"gvd_relattn error {rc}: {lib().gvd_relattn_last_error().decode()}")
-    return rc
+def ext():
+    """The compiled operator (csrc/relattn_torch_ext.cpp: forward and backward as one torch::autograd::Function) over the same library instance."""
+    global _EXT
+    if _EXT is None:
+        lib()
+        if not os.path.exists(_EXT_PATH):
+            raise RuntimeError(f"{_EXT_PATH} is missing: build the extensions first (python -c 'import __graft_entry__ as g; g.build()')")
+        spec = importlib.util.spec_from_file_location("_gvd_relattn_torch", _EXT_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.init(_LIB_PATH)
+        _EXT = mod
+    return _EXT
 
 
 @functools.lru_cache(maxsize=64)
@@ -64,9 +66,8 @@ def first_distances(side, max_distance):
 
 
 @functools.lru_cache(maxsize=64)
-def _first_array(side, max_distance):
-    f = first_distances(side, max_distance)
-    return (ctypes.c_int * len(f))(*f)
+def _first_tensor(side, max_distance):
+    return torch.tensor(first_distances(side, max_distance), dtype=torch.int32)
 
 
 def relative_buckets(distance, buckets, max_distance=128, bidirectional=True):
@@ -106,83 +107,6 @@ def relative_bias_attention_math(q, k, v, table, heads, *, max_distance=128, bid
     return out.transpose(0, 1).contiguous() if frame_major else out
 
 
-def _problem(q, k, v, out, table, heads, cfg):
-    """The C struct of a call; q, k, v, out as they will be read (k and v with the same strides)."""
-    max_distance, both, causal, q_start, kv_lens, scale, frame_major = cfg
-    bd, rd = (1, 0) if frame_major else (0, 1)
-    B, side = q.shape[bd], table.shape[0] // 2 if both else table.shape[0]
-    p = _Problem(B, heads, q.shape[rd], k.shape[rd], q.shape[-1] // heads, int(q.dtype == torch.bfloat16), _TYPES[table.dtype], table.shape[0], int(both),
-                 int(causal), _first_array(side, max_distance), scale)
-    if torch.is_tensor(q_start):
-        p.q_starts = q_start.data_ptr()
-    else:
-        p.q_start = q_start
-    if kv_lens is not None:
-        p.kv_lens = kv_lens.data_ptr()
-    (p.q_bs, p.q_rs), (p.kv_bs, p.kv_rs), (p.o_bs, p.o_rs) = (ops._view_strides(t, frame_major, B) for t in (q, k, out))
-    return p
-
-
-def _packed(t):
-    """t contiguous and 16-byte aligned (a contiguous view may begin anywhere)."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-def _workspace(n, like):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _forward(q, k, v, table, heads, cfg, want_lse):
-    frame_major = cfg[-1]
-    bd, rd = (1, 0) if frame_major else (0, 1)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[bd], heads, q.shape[rd]), dtype=torch.float32, device=q.device) if want_lse else None
-    if q.numel() == 0 or k.shape[rd] == 0:
-        return out.zero_(), lse
-    q, k, v = (t if ops._readable_in_place(t) else _packed(t) for t in (q, k, v))
-    B = q.shape[bd]
-    if ops._view_strides(k, frame_major, B) != ops._view_strides(v, frame_major, B):
-        k, v = _packed(k), _packed(v)
-    p = _problem(q, k, v, out, table, heads, cfg)
-    L = lib()
-    with ops._on(q.device):
-        ws = _workspace(_check(L.gvd_relattn_fwd_workspace(ctypes.byref(p))), q)
-        _check(L.gvd_relattn_fwd(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(ws), ops._stream()))
-    return out, lse
-
-
-class _RelativeBiasAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, table, heads, cfg):
-        q, k, v = _packed(q), _packed(k), _packed(v)
-        out, lse = _forward(q, k, v, table, heads, cfg, True)
-        ctx.save_for_backward(q, k, v, table, out, lse, cfg[4])
-        ctx.heads, ctx.cfg = heads, cfg
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        q, k, v, table, out, lse, kv_lens = ctx.saved_tensors
-        cfg = ctx.cfg[:4] + (kv_lens,) + ctx.cfg[5:]
-        dq, dk, dv, dtable = (torch.empty_like(t) for t in (q, k, v, table))
-        if q.numel() == 0 or k.numel() == 0:
-            return tuple(t.zero_() for t in (dq, dk, dv, dtable)) + (None, None)
-        g = _packed(g)
-        p = _problem(q, k, v, out, table, ctx.heads, cfg)
-        L = lib()
-        with ops._on(q.device):
-            ws = _workspace(_check(L.gvd_relattn_bwd_workspace(ctypes.byref(p))), q)
-            _check(L.gvd_relattn_bwd(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(),
-                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dtable.data_ptr(), ws.data_ptr(), ops._stream()))
-        return dq, dk, dv, dtable, None, None
-
-
 def _check_arguments(q, k, v, table, heads, bidirectional, q_start, kv_lens, scale, frame_major, max_distance):
     bad = lambda what: ValueError(f"relative_bias_attention: {what}")  # noqa: E731
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
@@ -213,19 +137,14 @@ def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirect
     """See ops.relative_bias_attention."""
     on_dev = ops._require_device(q, "relative_bias_attention")
     scale = (q.shape[-1] // max(heads, 1)) ** -0.5 if scale is None else float(scale)
+    starts = torch.is_tensor(q_start)
+    if (on_dev and q.dtype in (torch.float16, torch.bfloat16) and k.dtype is q.dtype and v.dtype is q.dtype and heads > 0 and q.shape[-1] == heads * 64
+            and 1e-30 < scale < 1e30 and (starts or -2 ** 29 <= q_start <= 2 ** 29)):
+        side = table.shape[0] // 2 if bidirectional else table.shape[0]
+        return ext().attend(q, k, v, table, heads, _first_tensor(side, max_distance), bidirectional, causal, 0 if starts else q_start, q_start if starts else None,
+                            kv_lens, scale, frame_major)
     _check_arguments(q, k, v, table, heads, bidirectional, q_start, kv_lens, scale, frame_major, max_distance)
-    if not (on_dev and q.dtype in (torch.float16, torch.bfloat16) and q.shape[-1] // heads == 64 and k.dtype == q.dtype and v.dtype == q.dtype):
-        if on_dev:
-            ops._torch_form("relative_bias_attention", f"dtypes {q.dtype}, {k.dtype}, {v.dtype}, head dim {q.shape[-1] // heads} (the MFMA kernels cover 16-bit heads of 64)")
-        return relative_bias_attention_math(q, k, v, table, heads, max_distance=max_distance, bidirectional=bidirectional, causal=causal, q_start=q_start,
-                                            kv_lens=kv_lens, scale=scale, frame_major=frame_major)
-    table = table.contiguous()
-    cfg = (int(max_distance), bool(bidirectional), bool(causal), q_start if torch.is_tensor(q_start) else int(q_start), kv_lens, scale, bool(frame_major))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
-        if torch.is_tensor(q_start):
-            raise NotImplementedError("relative_bias_attention: gradients with one q_start for the whole batch only (a tensor of them is for inference)")
-        bd = 1 if frame_major else 0
-        if k.shape[bd] != q.shape[bd]:   # one K / V for the whole batch: the backward addresses one per entry, autograd sums their gradients
-            k, v = (t.expand(*[q.shape[bd] if i == bd else -1 for i in range(3)]) for t in (k, v))
-        return _RelativeBiasAttention.apply(q, k, v, table, heads, cfg)
-    return _forward(q, k, v, table, heads, cfg, False)[0]
+    if on_dev:
+        ops._torch_form("relative_bias_attention", f"dtypes {q.dtype}, {k.dtype}, {v.dtype}, head dim {q.shape[-1] // heads} (the MFMA kernels cover 16-bit heads of 64)")
+    return relative_bias_attention_math(q, k, v, table, heads, max_distance=max_distance, bidirectional=bidirectional, causal=causal, q_start=q_start,
+                                        kv_lens=kv_lens, scale=scale, frame_major=frame_major)

@@ -5,6 +5,7 @@ import ctypes
 import math
 import os
 import re
+import struct
 
 import pytest
 import torch
@@ -15,6 +16,7 @@ from fused_optim import FusedAdamW
 gpu = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DEV = "cuda:0"
+TENSOR = struct.Struct("6Qq3fI")     # gvd_adamw_tensor, as a caller without torch binds it
 U = 2.0 ** -24      # half a step of float32, relative
 
 
@@ -72,15 +74,16 @@ def test_library_exports_every_declared_symbol():
 
 def test_c_entry_checks_its_arguments_before_any_launch():
     L = fused_optim.lib()
-    one = fused_optim._TENSOR.pack(0, 0, 0, 0, 0, 0, 5, 0.1, 1.0, 1.0, 0)
+    L.gvd_adamw_step.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 3 + [ctypes.c_void_p] * 2
+    one = TENSOR.pack(0, 0, 0, 0, 0, 0, 5, 0.1, 1.0, 1.0, 0)
     assert L.gvd_adamw_step(b"", 0, 0, 32, 0.9, 0.999, 1e-8, None, None) == 0
     for args, word in (((one, 1, 0, 32, 0.9, 0.999, 1e-8), b"null"), ((one, 1, 3, 32, 0.9, 0.999, 1e-8), b"param_type"), ((one, 1, 0, 16, 0.9, 0.999, 1e-8), b"state_bits"),
                        ((one, 1, 0, 32, 1.0, 0.999, 1e-8), b"betas"), ((one, 1, 0, 32, 0.9, float("nan"), 1e-8), b"betas"), ((one, 1, 0, 32, 0.9, 0.999, -1.0), b"eps"),
                        ((one, -1, 0, 32, 0.9, 0.999, 1e-8), b"bad")):
         assert L.gvd_adamw_step(*args, None, None) == -1 and word in L.gvd_optim_last_error(), (args, L.gvd_optim_last_error())
-    negative = fused_optim._TENSOR.pack(0, 0, 0, 0, 0, 0, -1, 0.1, 1.0, 1.0, 0)
+    negative = TENSOR.pack(0, 0, 0, 0, 0, 0, -1, 0.1, 1.0, 1.0, 0)
     assert L.gvd_adamw_step(negative, 1, 0, 32, 0.9, 0.999, 1e-8, None, None) == -1 and b"size" in L.gvd_optim_last_error()
-    empty = fused_optim._TENSOR.pack(0, 0, 0, 0, 0, 0, 0, 0.1, 1.0, 1.0, 0)
+    empty = TENSOR.pack(0, 0, 0, 0, 0, 0, 0, 0.1, 1.0, 1.0, 0)
     assert L.gvd_adamw_step(empty, 1, 0, 32, 0.9, 0.999, 1e-8, None, None) == 0      # nothing to do, nothing launched
     assert L.gvd_adamw_scalars(None, None, None, None, None, 1, ctypes.c_double(0.9), ctypes.c_double(0.999), 0, None, None) == -1
 

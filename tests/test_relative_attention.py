@@ -18,6 +18,13 @@ DEV = "cuda:0"
 D = 64
 
 
+class Problem(ctypes.Structure):       # gvd_relattn_problem, as a caller without torch binds it
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "H", "Nq", "Nk", "D", "is_bf16", "table_type", "buckets", "both", "causal")]
+                + [("first", ctypes.POINTER(ctypes.c_int)), ("scale", ctypes.c_float), ("q_start", ctypes.c_int), ("q_starts", ctypes.c_void_p),
+                   ("kv_lens", ctypes.c_void_p)]
+                + [(n, ctypes.c_longlong) for n in ("q_bs", "q_rs", "kv_bs", "kv_rs", "o_bs", "o_rs")])
+
+
 def bucket_plain(d, buckets, max_distance, both):
     side = buckets // 2 if both else buckets
     n = abs(d) if both else max(-d, 0)
@@ -136,7 +143,7 @@ def test_library_exports_every_declared_symbol():
         assert hasattr(relative.lib(), n), n
     body = hdr[hdr.index("typedef struct gvd_relattn_problem {"):hdr.index("} gvd_relattn_problem;")]
     members = [m for line in re.findall(r"^\s*(?:const )?(?:int|float|long long)\*? (.*);", body, flags=re.M) for m in re.findall(r"\w+", line)]
-    assert members == [n for n, _ in relative._Problem._fields_]
+    assert members == [n for n, _ in Problem._fields_]
 
 
 @pytest.mark.parametrize("side,max_distance", [(1, 2), (2, 8), (3, 16), (4, 64), (16, 128), (32, 128), (64, 500), (128, 1024)])
@@ -154,7 +161,7 @@ def problem(**kw):
     args = dict(B=1, H=2, Nq=40, Nk=50, D=64, is_bf16=0, table_type=0, buckets=8, both=1, causal=0, first=first, scale=0.125, q_start=0, q_bs=40 * 128, q_rs=128,
                 kv_bs=50 * 128, kv_rs=128, o_bs=40 * 128, o_rs=128)
     args.update(kw)
-    return relative._Problem(**args), first
+    return Problem(**args), first
 
 
 def test_c_entry_checks_its_arguments_before_any_launch():
@@ -163,7 +170,7 @@ def test_c_entry_checks_its_arguments_before_any_launch():
     assert L.gvd_relattn_fwd_workspace(ctypes.byref(p)) == 0 and L.gvd_relattn_bwd_workspace(ctypes.byref(p)) > 0
     assert L.gvd_relattn_fwd(ctypes.byref(p), *[None] * 8) == -1 and b"null" in L.gvd_relattn_last_error()
     assert L.gvd_relattn_bwd(ctypes.byref(p), *[None] * 13) == -1 and b"null" in L.gvd_relattn_last_error()
-    assert L.gvd_relattn_fwd(ctypes.byref(p), *[8] * 5, None, None, None) == -1 and b"aligned" in L.gvd_relattn_last_error()
+    assert L.gvd_relattn_fwd(ctypes.byref(p), *[ctypes.c_void_p(8)] * 5, None, None, None) == -1 and b"aligned" in L.gvd_relattn_last_error()
     odd, far = (ctypes.c_int * 4)(0, 2, 1, 9), (ctypes.c_int * 4)(0, 1, 2, 5000)
     for kw, word in ((dict(B=0), b"sizes"), (dict(Nk=0), b"sizes"), (dict(D=32), b"head dim"), (dict(buckets=7), b"even"), (dict(buckets=0), b"buckets"),
                      (dict(buckets=258), b"too many buckets"), (dict(first=odd), b"descend"), (dict(first=far), b"far"), (dict(scale=0.0), b"scale"),
@@ -172,11 +179,11 @@ def test_c_entry_checks_its_arguments_before_any_launch():
         bad, _keep = problem(**kw)
         assert L.gvd_relattn_fwd_workspace(ctypes.byref(bad)) == -1 and word in L.gvd_relattn_last_error(), (kw, L.gvd_relattn_last_error())
         assert L.gvd_relattn_bwd_workspace(ctypes.byref(bad)) == -1
-        assert L.gvd_relattn_fwd(ctypes.byref(bad), *[16] * 8) == -1 and L.gvd_relattn_bwd(ctypes.byref(bad), *[16] * 13) == -1
+        assert L.gvd_relattn_fwd(ctypes.byref(bad), *[ctypes.c_void_p(16)] * 8) == -1 and L.gvd_relattn_bwd(ctypes.byref(bad), *[ctypes.c_void_p(16)] * 13) == -1
     starts, _ = problem(q_starts=16)
-    assert L.gvd_relattn_bwd(ctypes.byref(starts), *[16] * 13) == -1 and b"q_start" in L.gvd_relattn_last_error()
+    assert L.gvd_relattn_bwd(ctypes.byref(starts), *[ctypes.c_void_p(16)] * 13) == -1 and b"q_start" in L.gvd_relattn_last_error()
     shared, _ = problem(B=2, kv_bs=0)
-    assert L.gvd_relattn_bwd(ctypes.byref(shared), *[16] * 13) == -1 and b"shared" in L.gvd_relattn_last_error()
+    assert L.gvd_relattn_bwd(ctypes.byref(shared), *[ctypes.c_void_p(16)] * 13) == -1 and b"shared" in L.gvd_relattn_last_error()
 
 
 @pytest.fixture
