@@ -5,7 +5,7 @@
 // Bound by memory: every element is read and written once -- 28 bytes with 32-bit moments and fp32 parameters, 16 with 8-bit ones -- and no
 // element depends on another (with 8-bit moments: on its block of 256).  So: one launch for up to MAX_TENSORS tensors (their table travels in
 // the kernel's arguments: nothing to upload, nothing that a captured graph could find changed), workgroups of CHUNK consecutive elements,
-// 16-byte accesses.
+// 16-byte accesses.  118M fp32 elements: 562 us, 5.9 TB/s (a plain copy of that size reaches 4.9); 11.8M with 8-bit moments: 34 us, 5.6 TB/s.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 (4 significant bits, 2^-9 .. 448) with one scale a block of 256 consecutive elements
 // (largest magnitude / 448), a block per wave.  Two choices carry this:
@@ -39,12 +39,12 @@ int fail(int code, const char* what, hipError_t e = hipSuccess)
 }
 
 constexpr int MAX_TENSORS = 52;   // 52 * 76 bytes and the other arguments: below 4 KiB of kernel arguments
-constexpr int CHUNK = 2048;       // elements a workgroup: eight blocks of 8-bit moments, two rounds of 256 lanes x 4
+constexpr int CHUNK = 2048;       // elements a workgroup: eight blocks of 8-bit moments, two rounds of 256 lanes x 4 (11.8M elements with 8-bit moments, ordinary accesses: 37.1 us; 1024 37.5, 4096 42.6)
 constexpr int BLOCK = GVD_ADAMW_BLOCK;
 
 struct Table {
     gvd_adamw_tensor t[MAX_TENSORS];
-    unsigned first[MAX_TENSORS];   // first workgroup of each tensor, ascending
+    unsigned first[MAX_TENSORS];   // first workgroup of each tensor, ascending; unused entries: the largest number
     int count;
 };
 
@@ -68,13 +68,15 @@ template <> struct Vec4<float> { typedef f4 type; };
 template <> struct Vec4<_Float16> { typedef h4 type; };
 template <> struct Vec4<__bf16> { typedef b4 type; };
 
-// Four consecutive elements as floats; beyond n: zeros.  `wide` (all pointers of the tensor aligned to a vector): one access where all four are there.
-template <typename T>
-__device__ __forceinline__ f4 load4(const T* __restrict__ p, long long i, long long n, bool wide)
+// Four consecutive elements as floats.  FULL: all of the workgroup's elements are there and every pointer is aligned to a vector; otherwise one by one,
+// zeros beyond n.  (Chosen once a workgroup, so the code of a full one has no branch around an access.)  Nothing is read twice: non-temporal accesses, 562 us
+// for 118M elements against 615 with ordinary ones (603 with the loads alone, 613 with the stores alone).
+template <bool FULL, typename T>
+__device__ __forceinline__ f4 load4(const T* __restrict__ p, long long i, long long n)
 {
     f4 r = { 0.f, 0.f, 0.f, 0.f };
-    if (wide && i + 4 <= n) {
-        const typename Vec4<T>::type x = *reinterpret_cast<const typename Vec4<T>::type*>(p + i);
+    if (FULL) {
+        const typename Vec4<T>::type x = __builtin_nontemporal_load(reinterpret_cast<const typename Vec4<T>::type*>(p + i));
 #pragma unroll
         for (int j = 0; j < 4; j++) r[j] = (float)x[j];
     } else {
@@ -85,14 +87,14 @@ __device__ __forceinline__ f4 load4(const T* __restrict__ p, long long i, long l
     return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* __restrict__ p, long long i, long long n, bool wide, f4 v)
+template <bool FULL, typename T>
+__device__ __forceinline__ void store4(T* __restrict__ p, long long i, long long n, f4 v)
 {
-    if (wide && i + 4 <= n) {
+    if (FULL) {
         typename Vec4<T>::type x;
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = (T)v[j];
-        *reinterpret_cast<typename Vec4<T>::type*>(p + i) = x;
+        __builtin_nontemporal_store(x, reinterpret_cast<typename Vec4<T>::type*>(p + i));
     } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -100,9 +102,10 @@ __device__ __forceinline__ void store4(T* __restrict__ p, long long i, long long
     }
 }
 
-__device__ __forceinline__ unsigned load4_bytes(const unsigned char* __restrict__ p, long long i, long long n, bool wide)
+template <bool FULL>
+__device__ __forceinline__ unsigned load4_bytes(const unsigned char* __restrict__ p, long long i, long long n)
 {
-    if (wide && i + 4 <= n) return *reinterpret_cast<const unsigned*>(p + i);
+    if (FULL) return *reinterpret_cast<const unsigned*>(p + i);
     unsigned r = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -110,9 +113,10 @@ __device__ __forceinline__ unsigned load4_bytes(const unsigned char* __restrict_
     return r;
 }
 
-__device__ __forceinline__ void store4_bytes(unsigned char* __restrict__ p, long long i, long long n, bool wide, unsigned v)
+template <bool FULL>
+__device__ __forceinline__ void store4_bytes(unsigned char* __restrict__ p, long long i, long long n, unsigned v)
 {
-    if (wide && i + 4 <= n) { *reinterpret_cast<unsigned*>(p + i) = v; return; }
+    if (FULL) { *reinterpret_cast<unsigned*>(p + i) = v; return; }
 #pragma unroll
     for (int j = 0; j < 4; j++)
         if (i + j < n) p[i + j] = (unsigned char)(v >> (8 * j));
@@ -129,38 +133,39 @@ __device__ __forceinline__ Step step_of(const Table& a, int k, const void* scala
     return { a.t[k].step_size, a.t[k].root_factor, a.t[k].keep, a.t[k].key };
 }
 
-// the tensor that workgroup `wg` belongs to: the last whose first workgroup is not behind it (uniform: scalar code)
+// The tensor that workgroup `wg` belongs to: the last whose first workgroup is not behind it.  All entries are compared (scalar code; unused ones are the
+// largest number): one trip to memory for the table, where a binary search makes one for each of its steps.
 __device__ __forceinline__ int tensor_of(const Table& a, unsigned wg)
 {
-    int lo = 0, hi = a.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.first[mid] <= wg) lo = mid; else hi = mid;
-    }
-    return lo;
+    int k = -1;
+#pragma unroll
+    for (int i = 0; i < MAX_TENSORS; i++) k += a.first[i] <= wg;
+    return k;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_adamw32(const Table a, float w1, float b2, float w2, float eps, const void* __restrict__ scalars)
+// p' from m', sqrt(v') and the step: the reciprocal is the unit's own (1 ulp), 2^-23 of an update.
+__device__ __forceinline__ float new_param(const Step& st, float p, float m, float root, float eps)
 {
-    const int k = tensor_of(a, blockIdx.x);
-    const gvd_adamw_tensor& t = a.t[k];
-    const Step st = step_of(a, k, scalars);
+    return st.keep * p - st.step_size * (m * __builtin_amdgcn_rcpf(root * st.root_factor + eps));
+}
+
+template <typename T, bool FULL>
+__device__ __forceinline__ void chunk32(const gvd_adamw_tensor& t, const Step& st, long long at, float w1, float b2, float w2, float eps)
+{
     T* __restrict__ p = (T*)t.param;
     const T* __restrict__ g = (const T*)t.grad;
     float* __restrict__ m = (float*)t.exp_avg;
     float* __restrict__ v = (float*)t.exp_avg_sq;
-    const long long n = t.n, at = (long long)(blockIdx.x - a.first[k]) * CHUNK + 4 * threadIdx.x;
-    const bool wide = (((uintptr_t)p | (uintptr_t)g) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 16) == 0;
+    const long long n = t.n;
     constexpr int R = CHUNK / 1024;
     f4 pp[R], gg[R], mm[R], vv[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {   // all loads of the workgroup's chunk in flight at once
         const long long i = at + 1024 * r;
-        gg[r] = load4(g, i, n, wide);
-        mm[r] = load4(m, i, n, wide);
-        vv[r] = load4(v, i, n, wide);
-        pp[r] = load4(p, i, n, wide);
+        gg[r] = load4<FULL>(g, i, n);
+        mm[r] = load4<FULL>(m, i, n);
+        vv[r] = load4<FULL>(v, i, n);
+        pp[r] = load4<FULL>(p, i, n);
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -171,62 +176,76 @@ __global__ void __launch_bounds__(256) k_adamw32(const Table a, float w1, float 
             const float gj = gg[r][j];
             mn[j] = mm[r][j] + w1 * (gj - mm[r][j]);
             vn[j] = b2 * vv[r][j] + w2 * (gj * gj);
-            pn[j] = st.keep * pp[r][j] - st.step_size * (mn[j] / (sqrtf(vn[j]) * st.root_factor + eps));
+            pn[j] = new_param(st, pp[r][j], mn[j], sqrtf(vn[j]), eps);
         }
-        store4(m, i, n, wide, mn);
-        store4(v, i, n, wide, vn);
-        store4(p, i, n, wide, pn);
+        store4<FULL>(m, i, n, mn);
+        store4<FULL>(v, i, n, vn);
+        store4<FULL>(p, i, n, pn);
     }
 }
-
-// x in [0, 448] as e4m3, rounded up with the probability of its distance from the lower neighbour (u: 16 random bits).  Scaled by 2^-120 a float's own
-// exponent and upper mantissa bits ARE the code, subnormals of the one becoming subnormals of the other; what is cut off is what the draw is added to.
-// least: the code that a value above 0 has at least.  What is not finite becomes e4m3's NaN.
-__device__ __forceinline__ unsigned to_e4m3(float x, unsigned u, unsigned least)
-{
-    const unsigned b = (__float_as_uint(fminf(x, 448.f) * 0x1p-120f) + (u << 4)) >> 20;
-    const unsigned c = b < least ? least : (b > 0x7eu ? 0x7eu : b);
-    return x < INFINITY ? c : 0x7fu;
-}
-
-__device__ __forceinline__ float wave_max(float x)
-{
-#pragma unroll
-    for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s, 64));
-    return x;
-}
-
-// The largest finite magnitude of four values.
-__device__ __forceinline__ float finite_max(f4 x)
-{
-    float r = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float y = fabsf(x[j]);
-        r = y < INFINITY ? fmaxf(r, y) : r;   // (also skips NaN)
-    }
-    return r;
-}
-
-// A block whose largest magnitude is below this is held as zeros: 1 / big would overflow.  (A root is never that small unless it is 0: the least
-// positive float's root is 3.7e-23.)
-constexpr float TINY = 0x1p-110f;
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_adamw8(const Table a, float w1, float b2, float w2, float eps, const void* __restrict__ scalars)
+__global__ void __launch_bounds__(256) k_adamw32(const Table a, float w1, float b2, float w2, float eps, const void* __restrict__ scalars)
 {
     const int k = tensor_of(a, blockIdx.x);
     const gvd_adamw_tensor& t = a.t[k];
     const Step st = step_of(a, k, scalars);
+    const long long begin = (long long)(blockIdx.x - a.first[k]) * CHUNK, at = begin + 4 * threadIdx.x;
+    const bool wide = (((uintptr_t)t.param | (uintptr_t)t.grad) % (4 * sizeof(T)) | ((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) % 16) == 0;
+    if (wide && begin + CHUNK <= t.n) chunk32<T, true>(t, st, at, w1, b2, w2, eps);
+    else chunk32<T, false>(t, st, at, w1, b2, w2, eps);
+}
+
+// x in [0, 448] as e4m3, rounded up with the probability of its distance from the lower neighbour (u: 16 random bits at 4 .. 19).  Scaled by 2^-120 a float's
+// own exponent and upper mantissa bits ARE the code, subnormals of the one becoming subnormals of the other; what is cut off is what the draw is added
+// to, and 448 plus a draw is still 448.  least: the code that a value above 0 has at least.
+__device__ __forceinline__ unsigned to_e4m3(float x, unsigned u, unsigned least)
+{
+    const unsigned b = (__float_as_uint(fminf(x, 448.f) * 0x1p-120f) + u) >> 20;
+    return b < least ? least : b;
+}
+
+// The largest of the wave's values, in all lanes (scalar): over rows of 16, then across the rows, without LDS.
+__device__ __forceinline__ unsigned wave_max(unsigned x)
+{
+#define GVD_STEP(ctrl, rows) { const unsigned y = __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false); x = x > y ? x : y; }
+    GVD_STEP(0x111, 0xf)   // row_shr:1
+    GVD_STEP(0x112, 0xf)   // row_shr:2
+    GVD_STEP(0x114, 0xf)   // row_shr:4
+    GVD_STEP(0x118, 0xf)   // row_shr:8
+    GVD_STEP(0x142, 0xa)   // row_bcast:15 into rows 1 and 3
+    GVD_STEP(0x143, 0xc)   // row_bcast:31 into rows 2 and 3
+#undef GVD_STEP
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Largest magnitude of a block as a float's bits (for values >= 0 they order as the values do); what is not finite lies above all that is.
+constexpr unsigned MAGNITUDE = 0x7fffffffu, NOT_FINITE = 0x7f800000u;
+__device__ __forceinline__ unsigned largest(f4 x, bool finite_only)
+{
+    unsigned r = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const unsigned y = __float_as_uint(x[j]) & MAGNITUDE;
+        if (!finite_only || y < NOT_FINITE) r = r > y ? r : y;
+    }
+    return wave_max(r);
+}
+
+// A block whose largest magnitude is below this is held as zeros: 1 / big would overflow.  (A root is never that small unless it is 0: the least positive
+// float's root is 3.7e-23.)
+constexpr float TINY = 0x1p-110f;
+
+template <typename T, bool FULL>
+__device__ __forceinline__ void chunk8(const gvd_adamw_tensor& t, const Step& st, long long at, int lane, float w1, float b2, float w2, float eps)
+{
     T* __restrict__ p = (T*)t.param;
     const T* __restrict__ g = (const T*)t.grad;
     unsigned char* __restrict__ m8 = (unsigned char*)t.exp_avg;
     unsigned char* __restrict__ r8 = (unsigned char*)t.exp_avg_sq;
     float* __restrict__ ms = t.exp_avg_scale;
     float* __restrict__ rs = t.exp_avg_sq_scale;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long n = t.n, at = (long long)(blockIdx.x - a.first[k]) * CHUNK + BLOCK * wave;
-    const bool wide = (((uintptr_t)p | (uintptr_t)g) % (4 * sizeof(T)) | ((uintptr_t)m8 | (uintptr_t)r8) % 4) == 0;
+    const long long n = t.n;
     constexpr int R = CHUNK / (4 * BLOCK);
     f4 pp[R], gg[R];
     unsigned mc[R], rc[R];
@@ -234,17 +253,17 @@ __global__ void __launch_bounds__(256) k_adamw8(const Table a, float w1, float b
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const long long base = at + 4 * BLOCK * r, i = base + 4 * lane;
-        gg[r] = load4(g, i, n, wide);
-        mc[r] = load4_bytes(m8, i, n, wide);
-        rc[r] = load4_bytes(r8, i, n, wide);
-        pp[r] = load4(p, i, n, wide);
-        sm[r] = base < n ? ms[base / BLOCK] : 0.f;
-        sr[r] = base < n ? rs[base / BLOCK] : 0.f;
+        gg[r] = load4<FULL>(g, i, n);
+        mc[r] = load4_bytes<FULL>(m8, i, n);
+        rc[r] = load4_bytes<FULL>(r8, i, n);
+        pp[r] = load4<FULL>(p, i, n);
+        sm[r] = FULL || base < n ? ms[base / BLOCK] : 0.f;
+        sr[r] = FULL || base < n ? rs[base / BLOCK] : 0.f;
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const long long base = at + 4 * BLOCK * r, i = base + 4 * lane;
-        if (base >= n) continue;   // (uniform over the wave)
+        if (!FULL && base >= n) continue;   // (uniform over the wave)
         const f4 m0 = { __builtin_amdgcn_cvt_f32_fp8(mc[r], 0), __builtin_amdgcn_cvt_f32_fp8(mc[r], 1),
                         __builtin_amdgcn_cvt_f32_fp8(mc[r], 2), __builtin_amdgcn_cvt_f32_fp8(mc[r], 3) };
         const f4 r0 = { __builtin_amdgcn_cvt_f32_fp8(rc[r], 0), __builtin_amdgcn_cvt_f32_fp8(rc[r], 1),
@@ -255,26 +274,46 @@ __global__ void __launch_bounds__(256) k_adamw8(const Table a, float w1, float b
             const float gj = gg[r][j], mj = m0[j] * sm[r], rj = r0[j] * sr[r];
             mn[j] = mj + w1 * (gj - mj);
             rn[j] = sqrtf(b2 * (rj * rj) + w2 * (gj * gj));
-            pn[j] = st.keep * pp[r][j] - st.step_size * (mn[j] / (rn[j] * st.root_factor + eps));
+            pn[j] = new_param(st, pp[r][j], mn[j], rn[j], eps);
         }
-        store4(p, i, n, wide, pn);
-        const float bm = wave_max(finite_max(mn)), br = wave_max(finite_max(rn));   // (elements beyond n: zeros)
-        const float fm = bm >= TINY ? 1.f / bm * 448.f : 0.f, fr = br >= TINY ? 1.f / br * 448.f : 0.f;
+        store4<FULL>(p, i, n, pn);
+        unsigned bm = largest(mn, false), br = largest(rn, false);   // (elements beyond n: zeros)
+        const bool odd = bm >= NOT_FINITE || br >= NOT_FINITE;
+        if (odd) { bm = largest(mn, true); br = largest(rn, true); }
+        // both scales at once: the moment's in the even lanes, the root's in the odd ones
+        const float big = __uint_as_float(lane & 1 ? br : bm);
+        const float scale = big >= TINY ? big * (1.f / 448.f) : 0.f, times = big >= TINY ? 1.f / big * 448.f : 0.f;
+        const float fm = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(times), 0)), fr = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(times), 1));
         unsigned cm = 0, cr = 0;
+        const unsigned h0 = (unsigned)i * 0x9D2C5681u + st.key;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const unsigned h = mix((unsigned)(i + j) * 0x9D2C5681u + st.key);
-            const unsigned c = to_e4m3(fabsf(mn[j]) * fm, h & 0xffffu, 0u);
-            cm |= (c | (mn[j] < 0.f ? 0x80u : 0u)) << (8 * j);
-            cr |= to_e4m3(rn[j] * fr, h >> 16, rn[j] > 0.f ? 1u : 0u) << (8 * j);
+            const unsigned h = mix(h0 + j * 0x9D2C5681u);
+            unsigned c = to_e4m3(fabsf(mn[j]) * fm, (h << 4) & 0xffff0u, 0u), d = to_e4m3(rn[j] * fr, (h >> 12) & 0xffff0u, rn[j] > 0.f ? 1u : 0u);
+            if (odd) {   // (uniform) what is not finite is held as e4m3's NaN
+                if ((__float_as_uint(mn[j]) & MAGNITUDE) >= NOT_FINITE) c = 0x7fu;
+                if ((__float_as_uint(rn[j]) & MAGNITUDE) >= NOT_FINITE) d = 0x7fu;
+            }
+            cm |= (c | ((__float_as_uint(mn[j]) >> 24) & 0x80u)) << (8 * j);
+            cr |= d << (8 * j);
         }
-        store4_bytes(m8, i, n, wide, cm);
-        store4_bytes(r8, i, n, wide, cr);
-        if (lane == 0) {
-            ms[base / BLOCK] = bm >= TINY ? bm / 448.f : 0.f;
-            rs[base / BLOCK] = br >= TINY ? br / 448.f : 0.f;
-        }
+        store4_bytes<FULL>(m8, i, n, cm);
+        store4_bytes<FULL>(r8, i, n, cr);
+        if (lane < 2) (lane ? rs : ms)[base / BLOCK] = scale;
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_adamw8(const Table a, float w1, float b2, float w2, float eps, const void* __restrict__ scalars)
+{
+    const int k = tensor_of(a, blockIdx.x);
+    const gvd_adamw_tensor& t = a.t[k];
+    const Step st = step_of(a, k, scalars);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long begin = (long long)(blockIdx.x - a.first[k]) * CHUNK, at = begin + BLOCK * wave;
+    const bool wide = (((uintptr_t)t.param | (uintptr_t)t.grad) % (4 * sizeof(T)) | ((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) % 4) == 0;
+    if (wide && begin + CHUNK <= t.n) chunk8<T, true>(t, st, at, lane, w1, b2, w2, eps);
+    else chunk8<T, false>(t, st, at, lane, w1, b2, w2, eps);
 }
 
 struct Counters {
@@ -337,6 +376,7 @@ int gvd_adamw_step(const gvd_adamw_tensor* tensors, int count, int param_type, i
             wgs += more;
         }
         if (!wgs) continue;
+        for (int j = a.count; j < MAX_TENSORS; j++) a.first[j] = 0xffffffffu;
         const void* sc = scalars ? (const char*)scalars + 16 * (size_t)from : nullptr;
         const dim3 grid((unsigned)wgs);
 #define GVD_LAUNCH(K, T) hipLaunchKernelGGL(K<T>, grid, dim3(256), 0, stream, a, w1, b2, w2, e, sc)
