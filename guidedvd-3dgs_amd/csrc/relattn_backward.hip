@@ -3,13 +3,12 @@
 //     P = exp2(S - lse),  dV = P^T dO,  dP = dO V^T,  dS = P o (dP - delta),  delta_i = sum_j P_ij dP_ij
 //     dQ = scale dS K,  dK = scale dS^T Q,  dT[b, h] = sum of dS_ij over the (i, j) whose distance lies in bucket b
 //
-// General rows, three kernels in turn, no sum whose order could change:
-//   k_rel_delta   delta from dO . O: O was rounded, and so were the P that made it, so this delta is 2^-9 off (bf16) -- enough for 16-bit gradients, not for
-//                 a table's gradient in 32 bits: its sums cancel (a row's dS sums to 0)
-//   k_rel_dq      a wave = 32 queries; walks the keys; also sums each row's dS, which is exactly what delta was off by, and puts delta right
-//   k_rel_dkv     a wave = 32 keys; walks the queries; dS of the table from the corrected delta: by distance into an array of the wave's own in LDS (a 32 x 32 block
-//                 adds its rows one half wave at a time: all lanes at different distances), blocks beyond the last border into one register; at the end
-//                 distances are summed into buckets, one row of partial sums a workgroup
+// General rows, kernels in turn, no sum whose order could change:
+//   k_rel_dq      a wave = 32 queries; delta from dO . O: O was rounded, and so were the P that made it, so this delta is 2^-9 off (bf16) -- enough for 16-bit
+//                 gradients, not for a table's gradient in 32 bits: its sums cancel (a row's dS sums to 0).  Walks the keys, and also sums each row's dS, which is
+//                 exactly what delta was off by: the delta that it leaves for k_rel_dkv is right
+//   k_rel_dkv     a wave = 32 keys; walks the queries; dS of the table from the corrected delta: by distance into an array of the wave's own in LDS, blocks beyond
+//                 the last border into one register; at the end distances are summed into buckets, one row of partial sums a workgroup
 //   k_rel_table   sums the partial rows, 64 bits
 // Up to 32 queries and keys: k_rel_short_bwd, a wave an item as in the forward; the wave's head is fixed, so dS is summed over its items in registers and goes
 // into buckets once.
@@ -19,65 +18,19 @@ using namespace gvdr;
 
 namespace {
 
+// A tile of 64 rows x 64 channels through 512 lanes, 16 bytes each: eight lanes a row.  Rows at or behind n_rows: the last one again (n_rows >= 1), and zeros in LDS.
 template <typename T>
-__global__ void __launch_bounds__(256) k_rel_delta(const Geo g, const T* __restrict__ o, const T* __restrict__ d_o, float* __restrict__ delta, long long rows)
+__device__ __forceinline__ typename Tr<T>::vec8 tile_load(const T* __restrict__ src, size_t rs, int row0, int n_rows, int tid)
 {
-    typedef typename Tr<T>::vec8 vec8;
-    const long long i = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);   // (b H + h) Nq + n; 8 lanes a row
-    if (i >= rows) return;
-    const long long bh = i / g.Nq;
-    const int n = (int)(i - bh * g.Nq), b = (int)(bh / g.H), h = (int)(bh - (long long)b * g.H);
-    const size_t off = (size_t)b * g.o_bs + (size_t)n * g.o_rs + (size_t)h * 64 + 8 * (threadIdx.x & 7);
-    const vec8 x = *reinterpret_cast<const vec8*>(o + off), y = *reinterpret_cast<const vec8*>(d_o + off);
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) s = fmaf((float)x[j], (float)y[j], s);
-    s += __shfl_xor(s, 1, 64);
-    s += __shfl_xor(s, 2, 64);
-    s += __shfl_xor(s, 4, 64);
-    if ((threadIdx.x & 7) == 0) delta[i] = s;
+    const int row = row0 + (tid >> 3);
+    return *reinterpret_cast<const typename Tr<T>::vec8*>(src + (size_t)(row < n_rows ? row : n_rows - 1) * rs + (tid & 7) * 8);
 }
 
-// A tile of 64 rows x 64 channels: registers, then LDS row-major and (TRANSPOSED) channel-major with two rows a dword.  Loads are unconditional (the last valid row
-// again; n_rows >= 1) and committed as zeros beyond n_rows.
-template <typename T> struct TileRegs { typename Tr<T>::vec8 r[2], t0, t1; };
-
-template <typename T, bool TRANSPOSED>
-__device__ __forceinline__ void tile_load(const T* __restrict__ src, size_t rs, int row0, int n_rows, int tid, TileRegs<T>& R)
+template <typename T>
+__device__ __forceinline__ void tile_commit(typename Tr<T>::vec8 x, int row0, int n_rows, int tid, T (*dst)[LDS_ROW])
 {
-    typedef typename Tr<T>::vec8 vec8;
-    const int last = n_rows - 1;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int c = tid + i * 256, g = row0 + (c >> 3);
-        R.r[i] = *reinterpret_cast<const vec8*>(src + (size_t)(g < last ? g : last) * rs + (c & 7) * 8);
-    }
-    if (TRANSPOSED) {
-        const int g = row0 + 2 * (tid & 31), c8 = (tid >> 5) * 8;
-        R.t0 = *reinterpret_cast<const vec8*>(src + (size_t)(g < last ? g : last) * rs + c8);
-        R.t1 = *reinterpret_cast<const vec8*>(src + (size_t)(g + 1 < last ? g + 1 : last) * rs + c8);
-    }
-}
-
-template <typename T, bool TRANSPOSED>
-__device__ __forceinline__ void tile_commit(int row0, int n_rows, int tid, const TileRegs<T>& R, T (*sRow)[LDS_ROW], T (*sTr)[LDS_ROW])
-{
-    typedef typename Tr<T>::vec8 vec8;
-    typedef T T2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int c = tid + i * 256, row = c >> 3;
-        *reinterpret_cast<vec8*>(&sRow[row][(c & 7) * 8]) = (row0 + row < n_rows) ? R.r[i] : vec8{};
-    }
-    if (TRANSPOSED) {
-        const int kp = tid & 31, c8 = (tid >> 5) * 8, g = row0 + 2 * kp;
-        const vec8 x0 = (g < n_rows) ? R.t0 : vec8{}, x1 = (g + 1 < n_rows) ? R.t1 : vec8{};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const T2 pr = { x0[i], x1[i] };
-            *reinterpret_cast<T2*>(&sTr[c8 + i][2 * kp]) = pr;
-        }
-    }
+    if (row0 + 64 > n_rows && row0 + (tid >> 3) >= n_rows) x = typename Tr<T>::vec8{};
+    *reinterpret_cast<typename Tr<T>::vec8*>(&dst[tid >> 3][(tid & 7) * 8]) = x;
 }
 
 // 64 channels of one row from a C-layout pair (x0: channels 0 .. 31, x1: 32 .. 63)
@@ -97,27 +50,46 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f16v& x0, c
     }
 }
 
+// Both kernels: 8 waves, two a SIMD.  Waves w and w + 4 share a block of 32 rows and take one half each of every 64-row tile of the other side; the second four hand
+// their sums over through LDS at the end, in registers' order.  Tiles are double-buffered: one barrier a tile, loads two tiles ahead.
+template <typename T> struct Tiles { T a[2][64][LDS_ROW], b[2][64][LDS_ROW]; };
+constexpr int HANDOVER = 4 * 32 * 64 * (int)sizeof(float);   // 4 waves x 32 registers x 64 lanes: fits the tiles' LDS
+static_assert(sizeof(Tiles<__bf16>) >= HANDOVER, "the hand-over uses the tiles' memory");
+
+__device__ __forceinline__ void hand_over(float* at, int wave, int lane, const f16v& x0, const f16v& x1)
+{
+    float* p = at + (wave & 3) * 2048 + lane;
+#pragma unroll
+    for (int r = 0; r < 16; r++) { p[64 * r] = x0[r]; p[64 * (16 + r)] = x1[r]; }
+}
+__device__ __forceinline__ void take_over(const float* at, int wave, int lane, f16v& x0, f16v& x1)
+{
+    const float* p = at + (wave & 3) * 2048 + lane;
+#pragma unroll
+    for (int r = 0; r < 16; r++) { x0[r] += p[64 * r]; x1[r] += p[64 * (16 + r)]; }
+}
+
 // ---- dQ, and delta put right ---------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ d_o, const float* __restrict__ lse,
-         float* __restrict__ delta, T* __restrict__ dq)
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ o, const T* __restrict__ d_o,
+         const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq)
 {
     typedef typename Tr<T>::vec8 vec8;
-    __shared__ __attribute__((aligned(16))) T sK[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sV[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sKt[64][LDS_ROW];
+    __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: K, b: V
+    __shared__ float sOff[4][32];
     extern __shared__ __attribute__((aligned(16))) float sBias[];
 
     int bh, tile_y;
     xcd_item_tile(bh, tile_y);
     const int b = bh / g.H, h = bh - b * g.H;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+    const int half = 32 * (wave >> 2);   // the half of each key tile
     const int start = start_of(g, b), len = len_of(g, b);
     const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64;
     const T* vb = v + (size_t)b * g.kv_bs + (size_t)h * 64;
-    const int q0 = tile_y * 128, query = q0 + wave * 32 + col, q_last = (q0 + 128 < g.Nq ? q0 + 128 : g.Nq) - 1;
-    const int first = start + q0 + wave * 32;   // position of the wave's first query
+    const int q0 = tile_y * 128, query = q0 + (wave & 3) * 32 + col, q_last = (q0 + 128 < g.Nq ? q0 + 128 : g.Nq) - 1;
+    const int first = start + q0 + (wave & 3) * 32;   // position of the wave's first query
     const int k_hi = g.causal ? clamp_int(start + q_last + 1, 0, len) : len;
     const int k_full = g.causal ? clamp_int(start + q0 + 1, 0, len) : len;
     const bool valid = query < g.Nq;
@@ -130,111 +102,126 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
         gf[ks] = *reinterpret_cast<const vec8*>(d_o + grow + 16 * ks + 8 * hi);
     }
     const float L = valid ? lse[(size_t)bh * g.Nq + query] : INFINITY;   // (infinite: every weight of the row is 0)
-    const float Dl = valid ? delta[(size_t)bh * g.Nq + query] : 0.f;
+    float Dl = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) {
+        const vec8 x = *reinterpret_cast<const vec8*>(o + grow + 16 * ks + 8 * hi);
+#pragma unroll
+        for (int j = 0; j < 8; j++) Dl = fmaf((float)x[j], (float)gf[ks][j], Dl);
+    }
+    Dl += __shfl_xor(Dl, 32, 64);
     f16v dq0 = {}, dq1 = {};
     float off = 0.f;   // this lane's part of the row's sum of dS
 
-    TileRegs<T> rk, rv;
+    vec8 rk = {}, rv = {};
     if (k_hi > 0) {
-        tile_load<T, true>(kb, (size_t)g.kv_rs, 0, len, tid, rk);
-        tile_load<T, false>(vb, (size_t)g.kv_rs, 0, len, tid, rv);
+        rk = tile_load(kb, (size_t)g.kv_rs, 0, len, tid);
+        rv = tile_load(vb, (size_t)g.kv_rs, 0, len, tid);
     }
-    fill_bias(g, h, sBias, tid, 256);
+    fill_bias(g, h, sBias, tid, 512);
+    if (k_hi > 0) {
+        tile_commit(rk, 0, len, tid, tiles.a[0]);
+        tile_commit(rv, 0, len, tid, tiles.b[0]);
+        if (64 < k_hi) {
+            rk = tile_load(kb, (size_t)g.kv_rs, 64, len, tid);
+            rv = tile_load(vb, (size_t)g.kv_rs, 64, len, tid);
+        }
+    }
     __syncthreads();
-    const float far_past = sBias[0], far_ahead = sBias[bias_len(g.reach) - 1];
-    for (int kt = 0; kt < k_hi; kt += 64) {
-        __syncthreads();
-        tile_commit<T, true>(kt, len, tid, rk, sK, sKt);
-        tile_commit<T, false>(kt, len, tid, rv, sV, nullptr);
+    const float far_past = sBias[0] * g.c, far_ahead = sBias[bias_len(g.reach) - 1] * g.c;
+    int buf = 0;
+    for (int kt = 0; kt < k_hi; kt += 64, buf ^= 1) {
         if (kt + 64 < k_hi) {
-            tile_load<T, true>(kb, (size_t)g.kv_rs, kt + 64, len, tid, rk);
-            tile_load<T, false>(vb, (size_t)g.kv_rs, kt + 64, len, tid, rv);
+            tile_commit(rk, kt + 64, len, tid, tiles.a[buf ^ 1]);
+            tile_commit(rv, kt + 64, len, tid, tiles.b[buf ^ 1]);
+            if (kt + 128 < k_hi) {
+                rk = tile_load(kb, (size_t)g.kv_rs, kt + 128, len, tid);
+                rv = tile_load(vb, (size_t)g.kv_rs, kt + 128, len, tid);
+            }
+        }
+        const int k0 = kt + half;   // the wave's 32 keys
+        f16v s = {}, dp = {};
+        float shift = -L;           // weights are exp2(s c + shift): a single bias of the block goes here
+        const bool past = k0 + 31 - first <= -g.reach, ahead = k0 - first - 31 >= g.reach;
+        if (past || ahead) shift += past ? far_past : far_ahead;
+        else {
+            const float* e = sBias + (k0 + 4 * hi - first - col + g.reach + PAD);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = e[(r & 3) + 8 * (r >> 2)];
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), qf[ks], s);
+            dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), gf[ks], dp);
+        }
+        if (k0 + 32 > k_full) {
+            const int seen = (g.causal && start + query + 1 < len ? start + query + 1 : len) - k0 - 4 * hi;
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
+        }
+        unsigned pd[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float d0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)) * (dp[2 * j] - Dl);
+            const float d1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift)) * (dp[2 * j + 1] - Dl);
+            off += d0 + d1;
+            pd[j] = Tr<T>::pack2(d0, d1);
+        }
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            const vec8 df = packed_c_to_b_operand<T>(pd, k2);
+            dq0 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), df, dq0);
+            dq1 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), df, dq1);
         }
         __syncthreads();
-        const bool masked = kt + 64 > k_full;
-        const bool far = kt + 63 - first <= -g.reach || kt - first - 31 >= g.reach;
-#pragma unroll
-        for (int kbk = 0; kbk < 2; kbk++) {
-            f16v s, dp = {};
-            if (far) {
-                const float x = kt < first ? far_past : far_ahead;
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = x;
-            } else {
-                const float* e = sBias + (kt + 32 * kbk + 4 * hi - first - col + g.reach + PAD);
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = e[(r & 3) + 8 * (r >> 2)];
-            }
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                const vec8 ak = *reinterpret_cast<const vec8*>(&sK[32 * kbk + col][16 * ks + 8 * hi]);
-                const vec8 av = *reinterpret_cast<const vec8*>(&sV[32 * kbk + col][16 * ks + 8 * hi]);
-                s = Tr<T>::mfma(ak, qf[ks], s);
-                dp = Tr<T>::mfma(av, gf[ks], dp);
-            }
-            if (masked) {
-                const int seen = (g.causal && start + query + 1 < len ? start + query + 1 : len) - kt - 32 * kbk - 4 * hi;
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
-            }
-            unsigned pd[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float d0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, -L)) * (dp[2 * j] - Dl);
-                const float d1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, -L)) * (dp[2 * j + 1] - Dl);
-                off += d0 + d1;
-                pd[j] = Tr<T>::pack2(d0, d1);
-            }
-#pragma unroll
-            for (int k2 = 0; k2 < 2; k2++) {
-                const vec8 df = packed_c_to_b_operand<T>(pd, k2);
-                const int kc = 32 * kbk + 16 * k2 + 8 * hi;
-                dq0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sKt[col][kc]), df, dq0);
-                dq1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sKt[32 + col][kc]), df, dq1);
-            }
-        }
     }
     off += __shfl_xor(off, 32, 64);
-    if (valid) {
-        store_row<T>(dq + qrow, dq0, dq1, g.scale, hi);
-        if (hi == 0) delta[(size_t)bh * g.Nq + query] = Dl + off;   // sum_j P dP = delta sum_j P + sum_j dS, and the weights sum to 1
+    float* at = reinterpret_cast<float*>(&tiles);
+    if (wave >= 4) {
+        hand_over(at, wave, lane, dq0, dq1);
+        if (hi == 0) sOff[wave & 3][col] = off;
+    }
+    __syncthreads();
+    if (wave < 4) {
+        take_over(at, wave, lane, dq0, dq1);
+        if (valid) {
+            store_row<T>(dq + qrow, dq0, dq1, g.scale, hi);
+            if (hi == 0) delta[(size_t)bh * g.Nq + query] = Dl + off + sOff[wave][col];   // sum_j P dP = delta sum_j P + sum_j dS, and the weights sum to 1
+        }
     }
 }
 
 // ---- dK, dV, and the table's partial sums ----------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ d_o, const float* __restrict__ lse,
           const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part)
 {
     typedef typename Tr<T>::vec8 vec8;
-    __shared__ __attribute__((aligned(16))) T sQ[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sdO[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sQt[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sdOt[64][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) float sLse[64];
-    __shared__ __attribute__((aligned(16))) float sDelta[64];
-    __shared__ float sFar[4][2];
-    extern __shared__ __attribute__((aligned(16))) float sBias[];   // the bias, then 4 arrays of sums by distance
+    __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: Q, b: dO
+    __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // lse and delta of a tile's rows
+    __shared__ float sFar[8][2];
+    __shared__ float sSkew[8][16 * 48];
+    extern __shared__ __attribute__((aligned(16))) float sBias[];   // the bias, then 8 arrays of sums by distance
     const int blen = bias_len(g.reach), span = g.reach + PAD;
 
     int bh, tile_y;
     xcd_item_tile(bh, tile_y);
     const int b = bh / g.H, h = bh - b * g.H;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+    const int half = 32 * (wave >> 2);   // the half of each query tile
     const int start = start_of(g, b), len = len_of(g, b);
     const T* qb = q + (size_t)b * g.q_bs + (size_t)h * 64;
     const T* gb = d_o + (size_t)b * g.o_bs + (size_t)h * 64;
     const size_t kvoff = (size_t)b * g.kv_bs + (size_t)h * 64;
-    const float* lse_b = lse + (size_t)bh * g.Nq;
-    const float* delta_b = delta + (size_t)bh * g.Nq;
+    const float* row_b = (wave == 0 ? lse : delta) + (size_t)bh * g.Nq;   // what waves 0 and 1 bring
 
-    const int k0 = tile_y * 128, kw = k0 + wave * 32, key = kw + col;
+    const int k0 = tile_y * 128, kw = k0 + (wave & 3) * 32, key = kw + col;
     const bool there = key < len;
     float* sums = sBias + blen * (1 + wave);
-    for (int e = tid; e < 4 * blen; e += 256) sBias[blen + e] = 0.f;
-    fill_bias(g, h, sBias, tid, 256);
+    float* skew = &sSkew[wave][4 * hi * 47 + col + 15];   // element (row i, key col) of 16 rows: 48 i + col - i + 15
+    const float* column = &sSkew[wave][lane < 47 ? lane : 47];
     vec8 kf[4], vf[4];
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
@@ -248,104 +235,104 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
 
     // queries that may see a key of this workgroup: all, or those at or behind its first key
     const int q_lo = k0 >= len ? g.Nq : (g.causal ? clamp_int(k0 - start, 0, g.Nq) / 64 * 64 : 0);
-    TileRegs<T> rq, rg;
-    float rl = 0.f, rd = 0.f;
+    vec8 rq = {}, rg = {};
+    float rr = 0.f;
     auto prefetch = [&](int qt) {
-        tile_load<T, true>(qb, (size_t)g.q_rs, qt, g.Nq, tid, rq);
-        tile_load<T, true>(gb, (size_t)g.o_rs, qt, g.Nq, tid, rg);
-        const int r = qt + (tid & 63) < g.Nq ? qt + (tid & 63) : g.Nq - 1;
-        rl = lse_b[r];
-        rd = delta_b[r];
+        rq = tile_load(qb, (size_t)g.q_rs, qt, g.Nq, tid);
+        rg = tile_load(gb, (size_t)g.o_rs, qt, g.Nq, tid);
+        if (wave < 2) rr = row_b[qt + lane < g.Nq ? qt + lane : g.Nq - 1];
+    };
+    auto commit = [&](int qt, int buf) {
+        tile_commit(rq, qt, g.Nq, tid, tiles.a[buf]);
+        tile_commit(rg, qt, g.Nq, tid, tiles.b[buf]);
+        if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? rr : (wave == 0 ? INFINITY : 0.f);   // rows past the end weigh 0
     };
     if (q_lo < g.Nq) prefetch(q_lo);
+    for (int e = tid; e < 8 * blen; e += 512) sBias[blen + e] = 0.f;
+    for (int e = lane; e < 16 * 48; e += 64) sSkew[wave][e] = 0.f;
+    fill_bias(g, h, sBias, tid, 512);
+    if (q_lo < g.Nq) {
+        commit(q_lo, 0);
+        if (q_lo + 64 < g.Nq) prefetch(q_lo + 64);
+    }
     __syncthreads();
-    const float far_past = sBias[0], far_ahead = sBias[blen - 1];
-    for (int qt = q_lo; qt < g.Nq; qt += 64) {
-        __syncthreads();
-        tile_commit<T, true>(qt, g.Nq, tid, rq, sQ, sQt);
-        tile_commit<T, true>(qt, g.Nq, tid, rg, sdO, sdOt);
-        if (tid < 64) {
-            const bool ok = qt + tid < g.Nq;
-            sLse[tid] = ok ? rl : INFINITY;   // rows past the end weigh 0
-            sDelta[tid] = ok ? rd : 0.f;
+    const float far_past = sBias[0] * g.c, far_ahead = sBias[blen - 1] * g.c;
+    int buf = 0;
+    for (int qt = q_lo; qt < g.Nq; qt += 64, buf ^= 1) {
+        if (qt + 64 < g.Nq) {
+            commit(qt + 64, buf ^ 1);
+            if (qt + 128 < g.Nq) prefetch(qt + 128);
         }
-        if (qt + 64 < g.Nq) prefetch(qt + 64);
-        __syncthreads();
+        const int first = start + qt + half;   // position of the block's first query
+        const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
+        f16v s = {}, dp = {};
+        float shift = 0.f;
+        const int e0 = key - first - 4 * hi + span - 27;   // row r of the block: e0 + 27 - (r & 3) - 8 (r >> 2)
+        if (past || ahead) shift = past ? far_past : far_ahead;
+        else {
 #pragma unroll
-        for (int sb = 0; sb < 2; sb++) {
-            const int first = start + qt + 32 * sb;   // position of the block's first query
-            const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
-            f16v s, dp = {};
-            const int e0 = key - first - 4 * hi + span - 27;   // row r of the block: e0 + 27 - (r & 3) - 8 (r >> 2)
-            if (past || ahead) {
-                const float x = past ? far_past : far_ahead;
+            for (int r = 0; r < 16; r++) s[r] = sBias[e0 + (27 - (r & 3) - 8 * (r >> 2))];
+        }
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = x;
-            } else {
+        for (int ks = 0; ks < 4; ks++) {
+            s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), kf[ks], s);
+            dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), vf[ks], dp);
+        }
+        if (kw + 32 > len || (g.causal && kw + 31 > first)) {
+            const int least = !there ? 0x7fffffff : (g.causal ? key - first - 4 * hi : -64);   // the key's first row that sees it
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = sBias[e0 + (27 - (r & 3) - 8 * (r >> 2))];
+            for (int r = 0; r < 16; r++)
+                if ((r & 3) + 8 * (r >> 2) < least) s[r] = -INFINITY;
+        }
+        float ds[16];
+        unsigned pp[8], pd[8];
+#pragma unroll
+        for (int g4 = 0; g4 < 4; g4++) {   // rows 8 g4 + 4 hi + {0 .. 3}
+            const f4v L = *reinterpret_cast<const f4v*>(&sRow[buf][0][half + 8 * g4 + 4 * hi]);
+            const f4v D = *reinterpret_cast<const f4v*>(&sRow[buf][1][half + 8 * g4 + 4 * hi]);
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                p[j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + j], g.c, shift - L[j]));
+                ds[4 * g4 + j] = p[j] * (dp[4 * g4 + j] - D[j]);
             }
+            pp[2 * g4] = Tr<T>::pack2(p[0], p[1]);
+            pp[2 * g4 + 1] = Tr<T>::pack2(p[2], p[3]);
+            pd[2 * g4] = Tr<T>::pack2(ds[4 * g4], ds[4 * g4 + 1]);
+            pd[2 * g4 + 1] = Tr<T>::pack2(ds[4 * g4 + 2], ds[4 * g4 + 3]);
+        }
+        if (past || ahead) {
+            float x = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                const vec8 aq = *reinterpret_cast<const vec8*>(&sQ[32 * sb + col][16 * ks + 8 * hi]);
-                const vec8 ag = *reinterpret_cast<const vec8*>(&sdO[32 * sb + col][16 * ks + 8 * hi]);
-                s = Tr<T>::mfma(aq, kf[ks], s);
-                dp = Tr<T>::mfma(ag, vf[ks], dp);
-            }
-            if (kw + 32 > len || (g.causal && kw + 31 > first)) {
-                const int least = !there ? 0x7fffffff : (g.causal ? key - first - 4 * hi : -64);   // the key's first row that sees it
+            for (int r = 0; r < 16; r++) x += ds[r];
+            if (past) far_sum[0] += x; else far_sum[1] += x;
+        } else {
+            // by distance: 16 rows at a time go into the wave's own rows of LDS, each shifted by its number, so that a distance is a column; a lane sums a column.
+            // (What a row leaves uncovered was zeroed once.  One addition in LDS an element instead: 6 us a tile, against 1.5 for all else.)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if ((r & 3) + 8 * (r >> 2) < least) s[r] = -INFINITY;
-            }
-            float ds[16];
-            unsigned pp[8], pd[8];
+            for (int x = 0; x < 2; x++) {
 #pragma unroll
-            for (int g4 = 0; g4 < 4; g4++) {   // rows 8 g4 + 4 hi + {0 .. 3}
-                const float4 L = *reinterpret_cast<const float4*>(&sLse[32 * sb + 8 * g4 + 4 * hi]);
-                const float4 D = *reinterpret_cast<const float4*>(&sDelta[32 * sb + 8 * g4 + 4 * hi]);
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + 0], g.c, -L.x)), p1 = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + 1], g.c, -L.y));
-                const float p2 = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + 2], g.c, -L.z)), p3 = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + 3], g.c, -L.w));
-                ds[4 * g4 + 0] = p0 * (dp[4 * g4 + 0] - D.x);
-                ds[4 * g4 + 1] = p1 * (dp[4 * g4 + 1] - D.y);
-                ds[4 * g4 + 2] = p2 * (dp[4 * g4 + 2] - D.z);
-                ds[4 * g4 + 3] = p3 * (dp[4 * g4 + 3] - D.w);
-                pp[2 * g4] = Tr<T>::pack2(p0, p1);
-                pp[2 * g4 + 1] = Tr<T>::pack2(p2, p3);
-                pd[2 * g4] = Tr<T>::pack2(ds[4 * g4], ds[4 * g4 + 1]);
-                pd[2 * g4 + 1] = Tr<T>::pack2(ds[4 * g4 + 2], ds[4 * g4 + 3]);
-            }
-            if (past || ahead) {
-                float x = 0.f;
+                for (int r = 0; r < 8; r++) skew[((r & 3) + 8 * (r >> 2)) * 47] = ds[8 * x + r];
+                wave_order();
+                float y = 0.f, z = 0.f;
 #pragma unroll
-                for (int r = 0; r < 16; r++) x += ds[r];
-                far_sum[past ? 0 : 1] += x;
-            } else {
-                // one half wave at a time: its 32 lanes are at 32 different distances; the other half's rows lie 4 further.  The array is this wave's own
-                // and LDS operations of a wave keep their order, so the sums do too.
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-                    if (hi == x) {
-#pragma unroll
-                        for (int r = 0; r < 16; r++) __hip_atomic_fetch_add(&sums[e0 + (27 - (r & 3) - 8 * (r >> 2))], ds[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-                    }
-            }
-#pragma unroll
-            for (int k2 = 0; k2 < 2; k2++) {
-                const vec8 pf = packed_c_to_b_operand<T>(pp, k2), df = packed_c_to_b_operand<T>(pd, k2);
-                const int qc = 32 * sb + 16 * k2 + 8 * hi;
-                dv0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sdOt[col][qc]), pf, dv0);
-                dv1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sdOt[32 + col][qc]), pf, dv1);
-                dk0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sQt[col][qc]), df, dk0);
-                dk1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sQt[32 + col][qc]), df, dk1);
+                for (int r = 0; r < 16; r += 2) { y += column[48 * r]; z += column[48 * (r + 1)]; }
+                if (lane < 47) sums[kw - first - 16 * x + lane - 15 + span] += y + z;
+                wave_order();
             }
         }
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            const vec8 pf = packed_c_to_b_operand<T>(pp, k2), df = packed_c_to_b_operand<T>(pd, k2);
+            dv0 = Tr<T>::mfma(transposed_operand(&tiles.b[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), pf, dv0);
+            dv1 = Tr<T>::mfma(transposed_operand(&tiles.b[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), pf, dv1);
+            dk0 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), df, dk0);
+            dk1 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), df, dk1);
+        }
+        __syncthreads();
     }
-    if (key < g.Nk) {   // (behind the length: zeros)
-        store_row<T>(dk + kvoff + (size_t)key * (size_t)g.kv_rs, dk0, dk1, g.scale, hi);
-        store_row<T>(dv + kvoff + (size_t)key * (size_t)g.kv_rs, dv0, dv1, 1.0f, hi);
-    }
-    // distances into buckets
+    float* at = reinterpret_cast<float*>(&tiles);
+    if (wave >= 4) hand_over(at, wave, lane, dk0, dk1);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         float x = far_sum[i];
@@ -354,25 +341,42 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         if (lane == 0) sFar[wave][i] = x;
     }
     __syncthreads();
-    for (int e = tid; e < blen; e += 256) sBias[e] = (sBias[blen + e] + sBias[2 * blen + e]) + (sBias[3 * blen + e] + sBias[4 * blen + e]);
+    if (wave < 4) {
+        take_over(at, wave, lane, dk0, dk1);
+        if (key < g.Nk) store_row<T>(dk + kvoff + (size_t)key * (size_t)g.kv_rs, dk0, dk1, g.scale, hi);   // (behind the length: zeros)
+    }
     __syncthreads();
-    if (tid < g.buckets) {
-        const int k_ = tid < g.side ? tid : tid - g.side;   // bucket within its direction: distances lo .. hi of it
-        const int lo = g.first[k_], up = k_ + 1 < g.side ? g.first[k_ + 1] - 1 : span;
-        const float past = (sFar[0][0] + sFar[1][0]) + (sFar[2][0] + sFar[3][0]), ahead = (sFar[0][1] + sFar[1][1]) + (sFar[2][1] + sFar[3][1]);
+    if (wave >= 4) hand_over(at, wave, lane, dv0, dv1);
+    // distances into buckets
+    for (int e = tid; e < blen; e += 512) {
         float x = 0.f;
-        if (tid < g.side) {
-            for (int n = lo; n <= up; n++) x += sBias[span - n];
-            if (tid == g.side - 1) x += past;
-            if (!g.both && tid == 0) {   // one direction: whatever lies ahead shares the bucket of distance 0
-                for (int n = 1; n <= span; n++) x += sBias[span + n];
-                x += ahead;
-            }
-        } else {
-            for (int n = lo > 1 ? lo : 1; n <= up; n++) x += sBias[span + n];
-            if (tid == g.buckets - 1) x += ahead;
-        }
-        part[((size_t)bh * gridDim.y + tile_y) * g.buckets + tid] = x;
+#pragma unroll
+        for (int w = 1; w <= 8; w++) x += sBias[w * blen + e];
+        sBias[e] = x;
+    }
+    __syncthreads();
+    if (wave < 4) {
+        take_over(at, wave, lane, dv0, dv1);
+        if (key < g.Nk) store_row<T>(dv + kvoff + (size_t)key * (size_t)g.kv_rs, dv0, dv1, 1.0f, hi);
+    }
+    float past = 0.f, ahead = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) { past += sFar[w][0]; ahead += sFar[w][1]; }
+    const int l16 = tid & 15;
+    for (int bucket = tid >> 4; bucket < g.buckets; bucket += 32) {   // 16 lanes a bucket
+        const bool fore = bucket >= g.side;
+        const int n_ = fore ? bucket - g.side : bucket;   // the bucket within its direction: distances lo .. up of it
+        const int lo = g.first[n_], up = n_ + 1 < g.side ? g.first[n_ + 1] - 1 : span;
+        float x = 0.f;
+        for (int n = lo + l16; n <= up; n += 16)
+            if (!fore || n > 0) x += sBias[fore ? span + n : span - n];
+        if (!g.both && bucket == 0)   // one direction: whatever lies ahead shares the bucket of distance 0
+            for (int n = 1 + l16; n <= span; n += 16) x += sBias[span + n];
+#pragma unroll
+        for (int w = 8; w; w >>= 1) x += __shfl_xor(x, w, 16);
+        if (bucket == g.side - 1) x += past;
+        if (bucket == (g.both ? g.buckets - 1 : 0)) x += ahead;
+        if (l16 == 0) part[((size_t)bh * gridDim.y + tile_y) * g.buckets + bucket] = x;
     }
 }
 
@@ -397,26 +401,21 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
                                                           float* __restrict__ part, int items, int waves)
 {
     typedef typename Tr<T>::vec8 vec8;
-    typedef T T2 __attribute__((ext_vector_type(2)));
-    constexpr int TP = 40, OP = 72;
-    __shared__ __attribute__((aligned(16))) T sQt[4][64][TP];
-    __shared__ __attribute__((aligned(16))) T sKt[4][64][TP];
-    __shared__ __attribute__((aligned(16))) T sGt[4][64][TP];
-    __shared__ __attribute__((aligned(16))) T sO[4][32][OP];
+    constexpr int OP = 72;
+    __shared__ __attribute__((aligned(16))) T sQ[4][32][OP];   // the item's rows, for the transposed operands
+    __shared__ __attribute__((aligned(16))) T sK[4][32][OP];
+    __shared__ __attribute__((aligned(16))) T sG[4][32][OP];
+    __shared__ __attribute__((aligned(16))) T sO[4][32][OP];   // results on their way out
     __shared__ __attribute__((aligned(16))) float sL[4][32];
     __shared__ __attribute__((aligned(16))) float sD[4][32];
-    __shared__ float sB[4][64];
-    __shared__ int sBk[4][64];
+    __shared__ float sB[4][64];   // (75776 bytes in all: two workgroups a CU)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, r32 = lane & 31;
     const int gw = blockIdx.x * 4 + wave;
     if (gw >= waves) return;   // (no barriers below)
     const int h = gw % g.H, step = waves / g.H, nb = items / g.H, start = start_of(g, 0);
     const int qr = r32 < g.Nq ? r32 : g.Nq - 1;
-    const int kp = lane & 15, vo = lane >> 4;
-    const int q0r = 2 * kp < g.Nq ? 2 * kp : g.Nq - 1, q1r = 2 * kp + 1 < g.Nq ? 2 * kp + 1 : g.Nq - 1;
-    sBk[wave][lane] = bucket_of(g, lane - 32 - start);
-    sB[wave][lane] = start_value(g, table_at(g, sBk[wave][lane], h));   // distances -32 .. 31 less the start
-    __builtin_amdgcn_wave_barrier();
+    sB[wave][lane] = start_value(g, table_at(g, bucket_of(g, lane - 32 - start), h));   // distances -32 .. 31 less the start
+    wave_order();
     const float* bias_q = &sB[wave][4 * hi - r32 + 32];        // key row r: + (r & 3) + 8 (r >> 2)
     const float* bias_k = &sB[wave][r32 - 4 * hi + 32 - 27];   // query row r: + 27 - (r & 3) - 8 (r >> 2)
     f16v acc = {};   // dS^T summed over the wave's items
@@ -437,38 +436,30 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
     };
     auto store_rows = [&](const f16v& x0, const f16v& x1, float mul, T* base, size_t rstride, int nrows) {
         store_row<T>(&sO[wave][r32][0], x0, x1, mul, hi);
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
 #pragma unroll
         for (int ps = 0; ps < 4; ps++) {
             const int row = (lane >> 3) + 8 * ps;
             const uint4 w = *reinterpret_cast<const uint4*>(&sO[wave][row][8 * (lane & 7)]);
             if (row < nrows) *reinterpret_cast<uint4*>(base + (size_t)row * rstride + 8 * (lane & 7)) = w;
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
     };
 
     load_ops(gw / g.H);
     for (int b = gw / g.H; b < nb; b += step) {
-        const int len = len_of(g, b), last = len > 0 ? len - 1 : 0;
-        const size_t qbase = (size_t)b * g.q_bs + (size_t)h * 64, gbase = (size_t)b * g.o_bs + (size_t)h * 64, kbase = (size_t)b * g.kv_bs + (size_t)h * 64;
-        const size_t k0r = (size_t)(2 * kp < last ? 2 * kp : last) * (size_t)g.kv_rs, k1r = (size_t)(2 * kp + 1 < last ? 2 * kp + 1 : last) * (size_t)g.kv_rs;
-        vec8 xq[2][2], xk[2][2], xg[2][2];
-#pragma unroll
-        for (int ps = 0; ps < 2; ps++) {
-            const int c = 8 * vo + 32 * ps;
-            xk[ps][0] = *reinterpret_cast<const vec8*>(k + kbase + k0r + c);
-            xk[ps][1] = *reinterpret_cast<const vec8*>(k + kbase + k1r + c);
-            xq[ps][0] = *reinterpret_cast<const vec8*>(q + qbase + (size_t)q0r * (size_t)g.q_rs + c);
-            xq[ps][1] = *reinterpret_cast<const vec8*>(q + qbase + (size_t)q1r * (size_t)g.q_rs + c);
-            xg[ps][0] = *reinterpret_cast<const vec8*>(d_o + gbase + (size_t)q0r * (size_t)g.o_rs + c);
-            xg[ps][1] = *reinterpret_cast<const vec8*>(d_o + gbase + (size_t)q1r * (size_t)g.o_rs + c);
-        }
+        const int len = len_of(g, b);
+        const size_t qbase = (size_t)b * g.q_bs + (size_t)h * 64, kbase = (size_t)b * g.kv_bs + (size_t)h * 64;
         const float L = r32 < g.Nq ? lse[((size_t)b * g.H + h) * g.Nq + qr] : INFINITY;   // (rows past the end weigh 0)
         if (len == 0) {   // row 0 was loaded, whatever it holds: a NaN times a weight of 0 would not be 0
 #pragma unroll
             for (int ks = 0; ks < 4; ks++) { kf[ks] = vec8{}; vf[ks] = vec8{}; }
+        }
 #pragma unroll
-            for (int ps = 0; ps < 2; ps++) { xk[ps][0] = vec8{}; xk[ps][1] = vec8{}; }
+        for (int ks = 0; ks < 4; ks++) {
+            *reinterpret_cast<vec8*>(&sQ[wave][r32][16 * ks + 8 * hi]) = qf[ks];
+            *reinterpret_cast<vec8*>(&sK[wave][r32][16 * ks + 8 * hi]) = kf[ks];
+            *reinterpret_cast<vec8*>(&sG[wave][r32][16 * ks + 8 * hi]) = gf[ks];
         }
         // ---- a query per lane ----
         f16v sT, dpT = {};
@@ -499,23 +490,13 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
             sL[wave][r32] = L;
             sD[wave][r32] = dl;
         }
-#pragma unroll
-        for (int ps = 0; ps < 2; ps++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int ch = (vo + 4 * ps) * 8 + i;
-                const T2 pk_ = { xk[ps][0][i], xk[ps][1][i] }, pq_ = { xq[ps][0][i], xq[ps][1][i] }, pg_ = { xg[ps][0][i], xg[ps][1][i] };
-                *reinterpret_cast<T2*>(&sKt[wave][ch][2 * kp]) = pk_;
-                *reinterpret_cast<T2*>(&sQt[wave][ch][2 * kp]) = pq_;
-                *reinterpret_cast<T2*>(&sGt[wave][ch][2 * kp]) = pg_;
-            }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         f16v a0 = {}, a1 = {};
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const vec8 df = packed_c_to_b_operand<T>(pdT, k2);
-            a0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sKt[wave][r32][16 * k2 + 8 * hi]), df, a0);
-            a1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sKt[wave][32 + r32][16 * k2 + 8 * hi]), df, a1);
+            a0 = Tr<T>::mfma(transposed_operand(&sK[wave][0][0], OP, 16 * k2, 0, lane), df, a0);
+            a1 = Tr<T>::mfma(transposed_operand(&sK[wave][0][0], OP, 16 * k2, 32, lane), df, a1);
         }
         // ---- a key per lane ----
         f16v s, dp = {};
@@ -547,30 +528,31 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const vec8 pf = packed_c_to_b_operand<T>(pp, k2), df = packed_c_to_b_operand<T>(pd, k2);
-            const int qc = 16 * k2 + 8 * hi;
-            dv0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sGt[wave][r32][qc]), pf, dv0);
-            dv1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sGt[wave][32 + r32][qc]), pf, dv1);
-            dk0 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sQt[wave][r32][qc]), df, dk0);
-            dk1 = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&sQt[wave][32 + r32][qc]), df, dk1);
+            dv0 = Tr<T>::mfma(transposed_operand(&sG[wave][0][0], OP, 16 * k2, 0, lane), pf, dv0);
+            dv1 = Tr<T>::mfma(transposed_operand(&sG[wave][0][0], OP, 16 * k2, 32, lane), pf, dv1);
+            dk0 = Tr<T>::mfma(transposed_operand(&sQ[wave][0][0], OP, 16 * k2, 0, lane), df, dk0);
+            dk1 = Tr<T>::mfma(transposed_operand(&sQ[wave][0][0], OP, 16 * k2, 32, lane), df, dk1);
         }
         store_rows(dv0, dv1, 1.0f, dv + kbase, (size_t)g.kv_rs, g.Nk);
         store_rows(dk0, dk1, g.scale, dk + kbase, (size_t)g.kv_rs, g.Nk);
     }
     // dS^T by distance (a lane each: 31 at most on either side), then by bucket
-    float* block = reinterpret_cast<float*>(&sO[wave][0][0]);   // [32 keys][33]
+    float* block = reinterpret_cast<float*>(&sO[wave][0][0]);   // [32 keys][33], then 64 buckets: 4480 of the wave's 4608 bytes
 #pragma unroll
     for (int r = 0; r < 16; r++) block[((r & 3) + 8 * (r >> 2) + 4 * hi) * 33 + r32] = acc[r];
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     float x = 0.f;
     for (int i = 0; i < 32; i++) {
         const int j = i + lane - 32;
         if (j >= 0 && j < 32) x += block[j * 33 + i];
     }
+    int* sBk = reinterpret_cast<int*>(block + 32 * 33);
     sB[wave][lane] = x;
-    __builtin_amdgcn_wave_barrier();
+    sBk[lane] = bucket_of(g, lane - 32 - start);
+    wave_order();
     for (int bucket = lane; bucket < g.buckets; bucket += 64) {
         float y = 0.f;
-        for (int e = 0; e < 64; e++) y += sBk[wave][e] == bucket ? sB[wave][e] : 0.f;
+        for (int e = 0; e < 64; e++) y += sBk[e] == bucket ? sB[wave][e] : 0.f;
         part[(size_t)gw * g.buckets + bucket] = y;
     }
 }
@@ -578,10 +560,10 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 bool is_short(const Geo& g) { return g.Nq <= 32 && g.Nk <= 32; }
 
-// waves of the short form: what stays resident (LDS: one workgroup of 4 a CU), a multiple of the heads
+// waves of the short form: what stays resident (LDS and registers: two workgroups of 4 a CU), a multiple of the heads
 int short_waves(const Geo& g, int B)
 {
-    long long waves = (long long)compute_units() * 4;
+    long long waves = (long long)compute_units() * 8;
     if (waves > (long long)B * g.H) waves = (long long)B * g.H;
     return (int)(waves >= g.H ? waves / g.H * g.H : g.H);
 }
@@ -593,7 +575,6 @@ int launch_bwd(const Geo& g, int B, const void* q, const void* k, const void* v,
                void* dtable, float* ws, hipStream_t stream)
 {
     const int BH = B * g.H;
-    const long long rows = (long long)BH * g.Nq;
     float* part = ws;
     float* delta = ws + partial_rows(g, B) * g.buckets;
     int tiles, count;
@@ -609,10 +590,9 @@ int launch_bwd(const Geo& g, int B, const void* q, const void* k, const void* v,
         if (BH > (1 << 23) || tiles > 65535 || qtiles > 65535 || (long long)B * tiles > 0x7fffffffLL) return fail(-1, "gvd_relattn_bwd: too many workgroups");
         count = B * tiles;
         const size_t lds = sizeof(float) * bias_len(g.reach);
-        hipLaunchKernelGGL(k_rel_delta<T>, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, stream, g, (const T*)out, (const T*)d_o, delta, rows);
-        hipLaunchKernelGGL(k_rel_dq<T>, dim3((unsigned)BH, (unsigned)qtiles), dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (const T*)d_o, lse, delta,
-                           (T*)dq);
-        hipLaunchKernelGGL(k_rel_dkv<T>, dim3((unsigned)BH, (unsigned)tiles), dim3(256), 5 * lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (const T*)d_o, lse,
+        hipLaunchKernelGGL(k_rel_dq<T>, dim3((unsigned)BH, (unsigned)qtiles), dim3(512), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (const T*)out,
+                           (const T*)d_o, lse, delta, (T*)dq);
+        hipLaunchKernelGGL(k_rel_dkv<T>, dim3((unsigned)BH, (unsigned)tiles), dim3(512), 9 * lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (const T*)d_o, lse,
                            (const float*)delta, (T*)dk, (T*)dv, part);
     }
     hipError_t e = hipGetLastError();

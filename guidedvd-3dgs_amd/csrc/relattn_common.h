@@ -30,7 +30,9 @@ __device__ __forceinline__ int bucket_of(const Geo& g, int d)
 {
     const int n = g.both ? (d < 0 ? -d : d) : (d < 0 ? -d : 0);
     int b = -1;
-    for (int k = 0; k < g.side; k++) b += g.first[k] <= n;
+    for (int k0 = 0; k0 < g.side; k0 += 16)   // (beyond side: the largest number)
+#pragma unroll
+        for (int k = 0; k < 16; k++) b += g.first[k0 + k] <= n;
     return b + (g.both && d > 0 ? g.side : 0);
 }
 
@@ -58,6 +60,35 @@ __device__ __forceinline__ void fill_bias(const Geo& g, int h, float* sBias, int
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 __device__ __forceinline__ int len_of(const Geo& g, int b) { return g.kv_lens ? clamp_int(g.kv_lens[b], 0, g.Nk) : g.Nk; }
 __device__ __forceinline__ int start_of(const Geo& g, int b) { return clamp_int(g.q_starts ? g.q_starts[b] : g.q_start, -(1 << 29), 1 << 29); }
+
+// The A operand of a 32x32x16 product from the TRANSPOSE of a row-major LDS tile: lane (m = lane & 31, hi) gets column c0 + m of rows k0 + 8 hi .. + 7.  One
+// transposing read hands each lane of a group of 16 one column of 4 rows x 16 columns, if lane s of the group points at row s / 4, columns 4 (s % 4) .. + 3.
+// (Writing tiles a second time, transposed, took 6 dword writes and 2 more loads a lane and tile.)
+template <typename T>
+__device__ __forceinline__ typename Tr<T>::vec8 transposed_operand(const T* tile, int pitch, int k0, int c0, int lane)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const T* p = tile + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * pitch + c0 + (lane & 16) + 4 * (lane & 3);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 4 * pitch));
+    return __builtin_bit_cast(typename Tr<T>::vec8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Between LDS writes of a wave and reads by its other lanes: LDS operations of a wave keep their order, so this only keeps the compiler's.
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Sum of two packed 16-bit values and acc in 32 bits: one instruction, and of the ROUNDED weights that the matrix unit multiplies.
+template <typename T> __device__ __forceinline__ float add_pair(unsigned packed, float acc)
+{
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    const T2 ones = { (T)1.0f, (T)1.0f };
+    if constexpr (std::is_same<T, _Float16>::value) return __builtin_amdgcn_fdot2(__builtin_bit_cast(T2, packed), ones, acc, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(T2, packed), ones, acc, false);
+}
 
 // Host side: checks a problem and fills a Geo (the table's pointer aside).
 int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who);

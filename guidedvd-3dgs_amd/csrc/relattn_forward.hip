@@ -75,15 +75,21 @@ int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who)
 namespace {
 
 // ---- general rows ------------------------------------------------------------------------------------------------------------
-template <typename T, int QB, bool PART>
+// The vector unit bounds this kernel: 32 exponentials a lane, query block and tile (quarter rate), against 16 products of the matrix unit.  So the loop does little else:
+//   * the maximum is not looked for: weights are formed with the running one, and a row sum above 2^15 (always for the first tile: the maximum starts
+//     below every score) sends the block through the exact path.  Numerators and denominator share the maximum, so any one that keeps weights finite
+//     gives the exact softmax;
+//   * each half wave keeps its own row sum, of the rounded weights (one dot product for two), or, where the backward will build on it (LSE), of the unrounded
+//     ones: its weights sum to 1 in 32 bits then, which the table's gradient needs; the halves meet at the end;
+//   * a block whose distances share one bias adds it to the exponent's shift, and its products start from the matrix unit's own zero.
+template <typename T, int QB, bool PART, bool LSE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
           float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
 {
     typedef typename Tr<T>::vec8 vec8;
-    typedef T T2 __attribute__((ext_vector_type(2)));
     __shared__ __attribute__((aligned(16))) T sKb[2][KV_TILE][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sVtb[2][64][LDS_ROW];
+    __shared__ __attribute__((aligned(16))) T sVb[2][KV_TILE][LDS_ROW];
     extern __shared__ __attribute__((aligned(16))) float sBias[];
 
     int bh, tile_y;
@@ -108,7 +114,7 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     int query[QB];
     vec8 qf[QB][4];
     f16v o0[QB], o1[QB];
-    float m[QB], l[QB];
+    float m[QB], l[QB];   // l: of this half wave's keys
 #pragma unroll
     for (int qi = 0; qi < QB; qi++) {
         query[qi] = q0 + (wave * QB + qi) * 32 + col;
@@ -121,32 +127,35 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         l[qi] = 0.f;
     }
 
-    // K and V tiles, two passes of 256 lanes: K rows as they are; V transposed, the two keys of a channel packed into a dword.  Rows at or behind `len`
-    // are zeros (whatever lies there, also NaN, meets a weight of 0); loads are unconditional (the last row again) and issued a tile ahead.
-    vec8 rk[2], rv0, rv1;
-    const int vkp = tid & 31, vc8 = (tid >> 5) * 8;
+    // K and V tiles as they are, 16 bytes a lane, two passes; loads are issued a tile ahead.  Rows at or behind `len` are zeros (whatever lies there, also NaN,
+    // meets a weight of 0): only the last tile looks.
+    vec8 rk[2], rv[2];
+    const int row = tid >> 3, c8 = (tid & 7) * 8;
+    const size_t lane_off = (size_t)row * (size_t)g.kv_rs + c8, half_off = 32 * (size_t)g.kv_rs;
     auto prefetch = [&](int kt) {
+        const size_t base = (size_t)kt * (size_t)g.kv_rs;
+        if (kt + KV_TILE <= len) {
 #pragma unroll
-        for (int ps = 0; ps < 2; ps++) {
-            const int c = tid + ps * 256, key = kt + (c >> 3);
-            rk[ps] = *reinterpret_cast<const vec8*>(kb + (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + (c & 7) * 8);
+            for (int ps = 0; ps < 2; ps++) {
+                rk[ps] = *reinterpret_cast<const vec8*>(kb + base + (lane_off + ps * half_off));
+                rv[ps] = *reinterpret_cast<const vec8*>(vb + base + (lane_off + ps * half_off));
+            }
+        } else {
+#pragma unroll
+            for (int ps = 0; ps < 2; ps++) {
+                const int key = kt + row + 32 * ps;
+                const size_t off = (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + c8;
+                rk[ps] = *reinterpret_cast<const vec8*>(kb + off);
+                rv[ps] = *reinterpret_cast<const vec8*>(vb + off);
+                if (key >= len) { rk[ps] = vec8{}; rv[ps] = vec8{}; }
+            }
         }
-        const int key = kt + 2 * vkp;
-        rv0 = *reinterpret_cast<const vec8*>(vb + (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + vc8);
-        rv1 = *reinterpret_cast<const vec8*>(vb + (size_t)(key + 1 < len ? key + 1 : len - 1) * (size_t)g.kv_rs + vc8);
     };
-    auto commit = [&](int kt, int buf) {
+    auto commit = [&](int buf) {
 #pragma unroll
         for (int ps = 0; ps < 2; ps++) {
-            const int c = tid + ps * 256, row = c >> 3;
-            *reinterpret_cast<vec8*>(&sKb[buf][row][(c & 7) * 8]) = kt + row < len ? rk[ps] : vec8{};
-        }
-        const int key = kt + 2 * vkp;
-        const vec8 x0 = key < len ? rv0 : vec8{}, x1 = key + 1 < len ? rv1 : vec8{};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const T2 pr = { x0[i], x1[i] };
-            *reinterpret_cast<T2*>(&sVtb[buf][vc8 + i][2 * vkp]) = pr;
+            *reinterpret_cast<vec8*>(&sKb[buf][row + 32 * ps][c8]) = rk[ps];
+            *reinterpret_cast<vec8*>(&sVb[buf][row + 32 * ps][c8]) = rv[ps];
         }
     };
     if (k_lo < k_hi) prefetch(k_lo);
@@ -156,103 +165,112 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     auto tile = [&](int kt, int buf, auto masked_tag) {
         constexpr bool MASKED = decltype(masked_tag)::value;
         if (kt + KV_TILE < k_hi) {
-            commit(kt + KV_TILE, buf ^ 1);
+            commit(buf ^ 1);
             if (kt + 2 * KV_TILE < k_hi) prefetch(kt + 2 * KV_TILE);
         }
         const T (*sK)[LDS_ROW] = sKb[buf];
-        const T (*sVt)[LDS_ROW] = sVtb[buf];
         f16v s0[QB], s1[QB];
-        auto scores = [&]() {
+        float far[QB];   // the single bias of a far block, in the exponent
+        vec8 a0[4], a1[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            a0[ks] = *reinterpret_cast<const vec8*>(&sK[col][16 * ks + 8 * hi]);
+            a1[ks] = *reinterpret_cast<const vec8*>(&sK[32 + col][16 * ks + 8 * hi]);
+        }
+#pragma unroll
+        for (int qi = 0; qi < QB; qi++) {
+            const int first = start + q0 + (wave * QB + qi) * 32;   // position of the block's first query (uniform)
+            if (kt + 63 - first <= -g.reach || kt - first - 31 >= g.reach) {
+                far[qi] = kt < first ? far_past : far_ahead;
+                s0[qi] = Tr<T>::mfma(a0[0], qf[qi][0], f16v{});
+                s1[qi] = Tr<T>::mfma(a1[0], qf[qi][0], f16v{});
+            } else {
+                far[qi] = 0.f;
+                const float* e = sBias + (kt + 4 * hi - first - col + g.reach + PAD);
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s0[qi][r] = e[(r & 3) + 8 * (r >> 2)];
+                    s1[qi][r] = e[(r & 3) + 8 * (r >> 2) + 32];
+                }
+                s0[qi] = Tr<T>::mfma(a0[0], qf[qi][0], s0[qi]);
+                s1[qi] = Tr<T>::mfma(a1[0], qf[qi][0], s1[qi]);
+            }
+        }
+#pragma unroll
+        for (int ks = 1; ks < 4; ks++)
 #pragma unroll
             for (int qi = 0; qi < QB; qi++) {
-                const int first = start + q0 + (wave * QB + qi) * 32;   // position of the block's first query (uniform)
-                if (kt + 63 - first <= -g.reach || kt - first - 31 >= g.reach) {
-                    const float x = kt < first ? far_past : far_ahead;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) { s0[qi][r] = x; s1[qi][r] = x; }
-                } else {
-                    const float* e = sBias + (kt + 4 * hi - first - col + g.reach + PAD);
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        s0[qi][r] = e[(r & 3) + 8 * (r >> 2)];
-                        s1[qi][r] = e[(r & 3) + 8 * (r >> 2) + 32];
-                    }
-                }
+                s0[qi] = Tr<T>::mfma(a0[ks], qf[qi][ks], s0[qi]);
+                s1[qi] = Tr<T>::mfma(a1[ks], qf[qi][ks], s1[qi]);
             }
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                const vec8 a0 = *reinterpret_cast<const vec8*>(&sK[col][16 * ks + 8 * hi]);
-                const vec8 a1 = *reinterpret_cast<const vec8*>(&sK[32 + col][16 * ks + 8 * hi]);
-#pragma unroll
-                for (int qi = 0; qi < QB; qi++) {
-                    s0[qi] = Tr<T>::mfma(a0, qf[qi][ks], s0[qi]);
-                    s1[qi] = Tr<T>::mfma(a1, qf[qi][ks], s1[qi]);
-                }
-            }
-            if (MASKED) {
-#pragma unroll
-                for (int qi = 0; qi < QB; qi++) {
-                    const int seen = (g.causal && start + query[qi] + 1 < len ? start + query[qi] + 1 : len) - kt - 4 * hi;
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int row = (r & 3) + 8 * (r >> 2);
-                        if (row >= seen) s0[qi][r] = -INFINITY;
-                        if (row + 32 >= seen) s1[qi][r] = -INFINITY;
-                    }
-                }
-            }
-        };
-        scores();
         unsigned pk0[QB][8], pk1[QB][8];
 #pragma unroll
         for (int qi = 0; qi < QB; qi++) {
-            float mt = fmaxf(s0[qi][0], s1[qi][0]);
+            if (MASKED) {
+                const int seen = (g.causal && start + query[qi] + 1 < len ? start + query[qi] + 1 : len) - kt - 4 * hi;
 #pragma unroll
-            for (int r = 1; r < 16; r++) mt = max3f(mt, s0[qi][r], s1[qi][r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float m_new = fmaxf(m[qi], mt * g.c);
-            const float alpha = __builtin_amdgcn_exp2f(m[qi] - m_new);
-            m[qi] = m_new;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j], g.c, -m_new)), p1 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j + 1], g.c, -m_new));
-                const float p2 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j], g.c, -m_new)), p3 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j + 1], g.c, -m_new));
-                pk0[qi][j] = Tr<T>::pack2(p0, p1);
-                pk1[qi][j] = Tr<T>::pack2(p2, p3);
-                sum += (p0 + p1) + (p2 + p3);
+                for (int r = 0; r < 16; r++) {
+                    if ((r & 3) + 8 * (r >> 2) >= seen) s0[qi][r] = -INFINITY;
+                    if ((r & 3) + 8 * (r >> 2) + 32 >= seen) s1[qi][r] = -INFINITY;
+                }
             }
-            l[qi] = fmaf(l[qi], alpha, sum + __shfl_xor(sum, 32, 64));
+            auto weights = [&]() {   // and this half's sum of them
+                const float shift = far[qi] - m[qi];
+                float x = 0.f, y = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; r++) { o0[qi][r] *= alpha; o1[qi][r] *= alpha; }
+                for (int j = 0; j < 8; j++) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j], g.c, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s0[qi][2 * j + 1], g.c, shift));
+                    const float p2 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j], g.c, shift)), p3 = __builtin_amdgcn_exp2f(fmaf(s1[qi][2 * j + 1], g.c, shift));
+                    pk0[qi][j] = Tr<T>::pack2(p0, p1);
+                    pk1[qi][j] = Tr<T>::pack2(p2, p3);
+                    x = LSE ? x + (p0 + p1) : add_pair<T>(pk0[qi][j], x);
+                    y = LSE ? y + (p2 + p3) : add_pair<T>(pk1[qi][j], y);
+                }
+                return x + y;
+            };
+            float sum = weights();
+            if (__any(!(sum <= 32768.f))) {   // (an infinity or a NaN too)
+                float mt = fmaxf(s0[qi][0], s1[qi][0]);
+#pragma unroll
+                for (int r = 1; r < 16; r++) mt = max3f(mt, s0[qi][r], s1[qi][r]);
+                mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+                const float m_new = fmaxf(m[qi], fmaf(mt, g.c, far[qi])), alpha = __builtin_amdgcn_exp2f(m[qi] - m_new);
+                m[qi] = m_new;
+                l[qi] *= alpha;
+#pragma unroll
+                for (int r = 0; r < 16; r++) { o0[qi][r] *= alpha; o1[qi][r] *= alpha; }
+                sum = weights();
+            }
+            l[qi] += sum;
         }
 #pragma unroll
         for (int kbk = 0; kbk < 2; kbk++)
 #pragma unroll
             for (int k2 = 0; k2 < 2; k2++) {
-                const int kcol = 32 * kbk + 16 * k2 + 8 * hi;
-                const vec8 a0 = *reinterpret_cast<const vec8*>(&sVt[col][kcol]);
-                const vec8 a1 = *reinterpret_cast<const vec8*>(&sVt[32 + col][kcol]);
+                const vec8 v0 = transposed_operand(&sVb[buf][0][0], LDS_ROW, 32 * kbk + 16 * k2, 0, lane);
+                const vec8 v1 = transposed_operand(&sVb[buf][0][0], LDS_ROW, 32 * kbk + 16 * k2, 32, lane);
 #pragma unroll
                 for (int qi = 0; qi < QB; qi++) {
                     const vec8 pf = packed_c_to_b_operand<T>(kbk == 0 ? pk0[qi] : pk1[qi], k2);
-                    o0[qi] = Tr<T>::mfma(a0, pf, o0[qi]);
-                    o1[qi] = Tr<T>::mfma(a1, pf, o1[qi]);
+                    o0[qi] = Tr<T>::mfma(v0, pf, o0[qi]);
+                    o1[qi] = Tr<T>::mfma(v1, pf, o1[qi]);
                 }
             }
         __syncthreads();
     };
 
     if (k_lo < k_hi) {   // (uniform over the workgroup)
-        commit(k_lo, 0);
+        commit(0);
         if (k_lo + KV_TILE < k_hi) prefetch(k_lo + KV_TILE);
         __syncthreads();
-        far_past = sBias[0];
-        far_ahead = sBias[bias_len(g.reach) - 1];
+        far_past = sBias[0] * g.c;
+        far_ahead = sBias[bias_len(g.reach) - 1] * g.c;
         int kt = k_lo, buf = 0;
         for (; kt < k_hi && kt + KV_TILE <= k_full; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::false_type{});
         for (; kt < k_hi; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::true_type{});
     }
+#pragma unroll
+    for (int qi = 0; qi < QB; qi++) l[qi] += __shfl_xor(l[qi], 32, 64);
 #pragma unroll
     for (int qi = 0; qi < QB; qi++) {
         if (query[qi] >= g.Nq) continue;
@@ -268,7 +286,7 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
             }
             continue;
         }
-        if (lse && hi == 0) lse[(size_t)bh * g.Nq + query[qi]] = l[qi] > 0.f ? m[qi] + __builtin_amdgcn_logf(l[qi]) : INFINITY;
+        if (LSE && hi == 0) lse[(size_t)bh * g.Nq + query[qi]] = l[qi] > 0.f ? m[qi] + __builtin_amdgcn_logf(l[qi]) : INFINITY;
         const float inv = l[qi] > 0.f ? 1.0f / l[qi] : 0.f;   // a row that sees nothing: zeros
         T* orow = out + (size_t)b * g.o_bs + (size_t)h * 64 + (size_t)query[qi] * (size_t)g.o_rs;
 #pragma unroll
@@ -285,33 +303,59 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     }
 }
 
-// Joins the parts of a row: 16 lanes a row, 4 channels each.
-template <typename T>
+// Joins the parts of a row: LN lanes a row, its 64 channels on 16 of them, LN / 16 parts at once.  64 lanes where rows are few (the trips to memory count: 16 x 10
+// rows in 13 parts 4.5 us, with 16 lanes 8.9), 16 where they are many (46080 rows in 3 parts 9.4 us, with 64 lanes 16.9).
+template <typename T, int LN>
 __global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __restrict__ part_o, const float2* __restrict__ part_ml, int parts, int BH,
                                                   T* __restrict__ out, float* __restrict__ lse)
 {
-    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long long)BH * g.Nq;
+    constexpr int CH = 64 / LN;   // parts come in CH rounds of LN: lane s of a round holds part s's maximum and sum (up to 64 parts)
+    const long long row = (long long)blockIdx.x * (256 / LN) + threadIdx.x / LN, rows = (long long)BH * g.Nq;
     if (row >= rows) return;
-    const int d0 = (threadIdx.x & 15) * 4;
-    float top = LOWEST;
-    for (int s = 0; s < parts; s++) top = fmaxf(top, part_ml[(size_t)s * rows + row].x);
-    float total = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < parts; s++) {
-        const float2 ml = part_ml[(size_t)s * rows + row];
-        const float w = __builtin_amdgcn_exp2f(ml.x - top);
-        const float4 x = *reinterpret_cast<const float4*>(part_o + ((size_t)s * rows + row) * 64 + d0);
-        total = fmaf(w, ml.y, total);
-        o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    const int lane = threadIdx.x % LN, d0 = (lane & 15) * 4;
+    float2 ml[CH];
+    float top = LOWEST, total = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int s = c * LN + lane;
+        ml[c] = s < parts ? part_ml[(size_t)s * rows + row] : make_float2(LOWEST, 0.f);
+        top = fmaxf(top, ml[c].x);
     }
-    const long long bh = row / g.Nq;
-    const int n = (int)(row - bh * g.Nq), b = (int)(bh / g.H), h = (int)(bh - (long long)b * g.H);
+#pragma unroll
+    for (int w = LN / 2; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, LN));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        if (c * LN >= parts) break;
+        const float weight = __builtin_amdgcn_exp2f(ml[c].x - top);
+        total = fmaf(weight, ml[c].y, total);
+        const int n = parts - c * LN < LN ? parts - c * LN : LN;
+        for (int s0 = 0; s0 < n; s0 += LN / 16) {
+            const int s = s0 + (lane >> 4);
+            const float w = __shfl(weight, s, LN);
+            if (s < n) {
+                const float4 x = *reinterpret_cast<const float4*>(part_o + ((size_t)(c * LN + s) * rows + row) * 64 + d0);
+                o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+            }
+        }
+    }
+#pragma unroll
+    for (int w = LN / 2; w; w >>= 1) total += __shfl_xor(total, w, LN);
+#pragma unroll
+    for (int w = 16; w < LN; w <<= 1) {
+        o.x += __shfl_xor(o.x, w, LN); o.y += __shfl_xor(o.y, w, LN);
+        o.z += __shfl_xor(o.z, w, LN); o.w += __shfl_xor(o.w, w, LN);
+    }
     const float inv = total > 0.f ? 1.0f / total : 0.f;
-    uint2 w;
-    w.x = Tr<T>::pack2(o.x * inv, o.y * inv);
-    w.y = Tr<T>::pack2(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(out + (size_t)b * g.o_bs + (size_t)n * g.o_rs + (size_t)h * 64 + d0) = w;
-    if (lse && d0 == 0) lse[row] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+    if (lane < 16) {
+        const long long bh = row / g.Nq;
+        const int n = (int)(row - bh * g.Nq), b = (int)(bh / g.H), h = (int)(bh - (long long)b * g.H);
+        uint2 w;
+        w.x = Tr<T>::pack2(o.x * inv, o.y * inv);
+        w.y = Tr<T>::pack2(o.z * inv, o.w * inv);
+        *reinterpret_cast<uint2*>(out + (size_t)b * g.o_bs + (size_t)n * g.o_rs + (size_t)h * 64 + d0) = w;
+        if (lse && lane == 0) lse[row] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+    }
 }
 
 // ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
@@ -358,10 +402,10 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
     int biased = 0x7fffffff;   // the start that `bias` is for
     auto set_bias = [&](int start) {
         sB[wave][lane] = start_value(g, table_at(g, bucket_of(g, lane - 32 - start), h));   // distances -32 .. 31 less the start
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
 #pragma unroll
         for (int r = 0; r < 16; r++) bias[r] = sB[wave][(r & 3) + 8 * (r >> 2) + 4 * hi - r32 + 32];
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         biased = start;
     };
     load(gw / g.H);
@@ -376,7 +420,7 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
                 const T2 pr = { va[ps][i], vb[ps][i] };
                 *reinterpret_cast<T2*>(&sVt[wave][(vo + 4 * ps) * 8 + i][2 * kp]) = pr;
             }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         f16v s = bias;
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) s = Tr<T>::mfma(kf[ks], qf[ks], s);
@@ -422,7 +466,7 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
             *reinterpret_cast<uint2*>(&sO[wave][r32][d0]) = w0;
             *reinterpret_cast<uint2*>(&sO[wave][r32][32 + d0]) = w1;
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         T* ob = out + (size_t)b * g.o_bs + (size_t)h * 64 + 8 * (lane & 7);
 #pragma unroll
         for (int ps = 0; ps < 4; ps++) {
@@ -430,7 +474,7 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
             const uint4 w = *reinterpret_cast<const uint4*>(&sO[wave][row][8 * (lane & 7)]);
             if (row < g.Nq) *reinterpret_cast<uint4*>(ob + (size_t)row * (size_t)g.o_rs) = w;
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
     }
 }
 
@@ -614,16 +658,23 @@ int launch_fwd(const Geo& g, int B, const void* q, const void* k, const void* v,
 #undef GVD_FEW
     } else {
         const dim3 grid((unsigned)BH, (unsigned)(pl.tiles * pl.parts));
-#define GVD_GEN(Q, P) hipLaunchKernelGGL((k_rel_fwd<T, Q, P>), grid, dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
-        if (pl.qb == 2) { if (pl.parts > 1) GVD_GEN(2, true); else GVD_GEN(2, false); }
-        else            { if (pl.parts > 1) GVD_GEN(1, true); else GVD_GEN(1, false); }
+#define GVD_GEN(Q, P) if (lse) GVD_GEN_(Q, P, true); else GVD_GEN_(Q, P, false)
+#define GVD_GEN_(Q, P, L) hipLaunchKernelGGL((k_rel_fwd<T, Q, P, L>), grid, dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
+        if (pl.qb == 2 && pl.parts > 1) { GVD_GEN(2, true); }
+        else if (pl.qb == 2) { GVD_GEN(2, false); }
+        else if (pl.parts > 1) { GVD_GEN(1, true); }
+        else { GVD_GEN(1, false); }
 #undef GVD_GEN
+#undef GVD_GEN_
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(-2, "launch k_rel_*", e);
     if (pl.parts > 1) {
         const long long rows = (long long)BH * g.Nq;
-        hipLaunchKernelGGL(k_rel_join<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, g, po, ml, pl.parts, BH, (T*)out, lse);
+        if (rows < 4096)
+            hipLaunchKernelGGL((k_rel_join<T, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, g, po, ml, pl.parts, BH, (T*)out, lse);
+        else
+            hipLaunchKernelGGL((k_rel_join<T, 16>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, g, po, ml, pl.parts, BH, (T*)out, lse);
         e = hipGetLastError();
         if (e != hipSuccess) return fail(-2, "launch k_rel_join", e);
     }
