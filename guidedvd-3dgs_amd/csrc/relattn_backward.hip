@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(64) k_rel_table(const float* __restrict__ part
 
 // ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
 // Both orientations of the score block are computed (a query per lane for dQ, delta and the table; a key per lane for dK and dV): 16 small products instead of a
-// transposition through LDS; delta = sum_j P dP directly, O is not read.
+// transposition of the weights; delta = sum_j P dP directly, O is not read.  Rows are read whole, 8 lanes each, and lie in LDS, where all operand forms come from;
+// V's place takes the results on their way out.  The next item's rows are requested as soon as this one's lie there.
 template <typename T>
 __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ d_o,
                                                           const float* __restrict__ lse, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
@@ -402,10 +403,10 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
 {
     typedef typename Tr<T>::vec8 vec8;
     constexpr int OP = 72;
-    __shared__ __attribute__((aligned(16))) T sQ[4][32][OP];   // the item's rows, for the transposed operands
+    __shared__ __attribute__((aligned(16))) T sQ[4][32][OP];
     __shared__ __attribute__((aligned(16))) T sK[4][32][OP];
     __shared__ __attribute__((aligned(16))) T sG[4][32][OP];
-    __shared__ __attribute__((aligned(16))) T sO[4][32][OP];   // results on their way out
+    __shared__ __attribute__((aligned(16))) T sV[4][32][OP];
     __shared__ __attribute__((aligned(16))) float sL[4][32];
     __shared__ __attribute__((aligned(16))) float sD[4][32];
     __shared__ float sB[4][64];   // (75776 bytes in all: two workgroups a CU)
@@ -413,62 +414,79 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
     const int gw = blockIdx.x * 4 + wave;
     if (gw >= waves) return;   // (no barriers below)
     const int h = gw % g.H, step = waves / g.H, nb = items / g.H, start = start_of(g, 0);
-    const int qr = r32 < g.Nq ? r32 : g.Nq - 1;
+    const int row = lane >> 3, c8 = 8 * (lane & 7);   // rows 8 i + row
     sB[wave][lane] = start_value(g, table_at(g, bucket_of(g, lane - 32 - start), h));   // distances -32 .. 31 less the start
     wave_order();
     const float* bias_q = &sB[wave][4 * hi - r32 + 32];        // key row r: + (r & 3) + 8 (r >> 2)
     const float* bias_k = &sB[wave][r32 - 4 * hi + 32 - 27];   // query row r: + 27 - (r & 3) - 8 (r >> 2)
     f16v acc = {};   // dS^T summed over the wave's items
 
-    vec8 qf[4], kf[4], vf[4], gf[4];
-    auto load_ops = [&](int b) {
-        const int n = len_of(g, b), last = n > 0 ? n - 1 : 0;
-        const T* qb = q + (size_t)b * g.q_bs + (size_t)h * 64 + (size_t)qr * (size_t)g.q_rs + 8 * hi;
-        const T* gb = d_o + (size_t)b * g.o_bs + (size_t)h * 64 + (size_t)qr * (size_t)g.o_rs + 8 * hi;
-        const size_t kvb = (size_t)b * g.kv_bs + (size_t)h * 64 + (size_t)(r32 < last ? r32 : last) * (size_t)g.kv_rs + 8 * hi;
+    vec8 rq[4], rk[4], rv[4], rg[4];
+    float L_next;
+    int len_next;
+    auto load_kv = [&](int b) {
+        len_next = len_of(g, b);
+        const int last = len_next > 0 ? len_next - 1 : 0;
+        const size_t kv = (size_t)b * g.kv_bs + (size_t)h * 64 + c8;
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            qf[ks] = *reinterpret_cast<const vec8*>(qb + 16 * ks);
-            kf[ks] = *reinterpret_cast<const vec8*>(k + kvb + 16 * ks);
-            vf[ks] = *reinterpret_cast<const vec8*>(v + kvb + 16 * ks);
-            gf[ks] = *reinterpret_cast<const vec8*>(gb + 16 * ks);
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + row;
+            const size_t j = r < last ? r : last;
+            rk[i] = *reinterpret_cast<const vec8*>(k + kv + j * (size_t)g.kv_rs);
+            rv[i] = *reinterpret_cast<const vec8*>(v + kv + j * (size_t)g.kv_rs);
         }
     };
+    auto load_q = [&](int b) {
+        const size_t qb = (size_t)b * g.q_bs + (size_t)h * 64 + c8, gb = (size_t)b * g.o_bs + (size_t)h * 64 + c8;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + row;
+            const size_t n = r < g.Nq ? r : g.Nq - 1;
+            rq[i] = *reinterpret_cast<const vec8*>(q + qb + n * (size_t)g.q_rs);
+            rg[i] = *reinterpret_cast<const vec8*>(d_o + gb + n * (size_t)g.o_rs);
+        }
+        L_next = lse[((size_t)b * g.H + h) * g.Nq + (r32 < g.Nq ? r32 : g.Nq - 1)];
+    };
+    auto operand = [&](const T (&x)[32][OP], int ks) { return *reinterpret_cast<const vec8*>(&x[r32][16 * ks + 8 * hi]); };
     auto store_rows = [&](const f16v& x0, const f16v& x1, float mul, T* base, size_t rstride, int nrows) {
-        store_row<T>(&sO[wave][r32][0], x0, x1, mul, hi);
+        store_row<T>(&sV[wave][r32][0], x0, x1, mul, hi);
         wave_order();
 #pragma unroll
-        for (int ps = 0; ps < 4; ps++) {
-            const int row = (lane >> 3) + 8 * ps;
-            const uint4 w = *reinterpret_cast<const uint4*>(&sO[wave][row][8 * (lane & 7)]);
-            if (row < nrows) *reinterpret_cast<uint4*>(base + (size_t)row * rstride + 8 * (lane & 7)) = w;
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + row;
+            const u4 w = *reinterpret_cast<const u4*>(&sV[wave][r][c8]);
+            if (r < nrows) __builtin_nontemporal_store(w, reinterpret_cast<u4*>(base + (size_t)r * rstride + c8));
         }
         wave_order();
     };
 
-    load_ops(gw / g.H);
+    load_kv(gw / g.H);
+    load_q(gw / g.H);
     for (int b = gw / g.H; b < nb; b += step) {
-        const int len = len_of(g, b);
+        const int len = len_next;
         const size_t qbase = (size_t)b * g.q_bs + (size_t)h * 64, kbase = (size_t)b * g.kv_bs + (size_t)h * 64;
-        const float L = r32 < g.Nq ? lse[((size_t)b * g.H + h) * g.Nq + qr] : INFINITY;   // (rows past the end weigh 0)
+        const float L = r32 < g.Nq ? L_next : INFINITY;   // (rows past the end weigh 0)
         if (len == 0) {   // row 0 was loaded, whatever it holds: a NaN times a weight of 0 would not be 0
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) { kf[ks] = vec8{}; vf[ks] = vec8{}; }
+            for (int i = 0; i < 4; i++) { rk[i] = vec8{}; rv[i] = vec8{}; }
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            *reinterpret_cast<vec8*>(&sQ[wave][r32][16 * ks + 8 * hi]) = qf[ks];
-            *reinterpret_cast<vec8*>(&sK[wave][r32][16 * ks + 8 * hi]) = kf[ks];
-            *reinterpret_cast<vec8*>(&sG[wave][r32][16 * ks + 8 * hi]) = gf[ks];
+        for (int i = 0; i < 4; i++) {
+            *reinterpret_cast<vec8*>(&sK[wave][8 * i + row][c8]) = rk[i];
+            *reinterpret_cast<vec8*>(&sQ[wave][8 * i + row][c8]) = rq[i];
+            *reinterpret_cast<vec8*>(&sV[wave][8 * i + row][c8]) = rv[i];
+            *reinterpret_cast<vec8*>(&sG[wave][8 * i + row][c8]) = rg[i];
         }
+        load_kv(b + step < nb ? b + step : b);   // in flight under everything below
+        wave_order();
         // ---- a query per lane ----
         f16v sT, dpT = {};
 #pragma unroll
         for (int r = 0; r < 16; r++) sT[r] = bias_q[(r & 3) + 8 * (r >> 2)];
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
-            sT = Tr<T>::mfma(kf[ks], qf[ks], sT);
-            dpT = Tr<T>::mfma(vf[ks], gf[ks], dpT);
+            sT = Tr<T>::mfma(operand(sK[wave], ks), operand(sQ[wave], ks), sT);
+            dpT = Tr<T>::mfma(operand(sV[wave], ks), operand(sG[wave], ks), dpT);
         }
         const int seen = (g.causal && start + r32 + 1 < len ? start + r32 + 1 : len) - 4 * hi;
         float p[16], dl = 0.f;
@@ -504,10 +522,11 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
         for (int r = 0; r < 16; r++) s[r] = bias_k[27 - (r & 3) - 8 * (r >> 2)];
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
-            s = Tr<T>::mfma(qf[ks], kf[ks], s);
-            dp = Tr<T>::mfma(gf[ks], vf[ks], dp);
+            s = Tr<T>::mfma(operand(sQ[wave], ks), operand(sK[wave], ks), s);
+            dp = Tr<T>::mfma(operand(sG[wave], ks), operand(sV[wave], ks), dp);
         }
-        load_ops(b + step < nb ? b + step : b);   // in flight under everything below
+        load_q(b + step < nb ? b + step : b);
+        wave_order();
         store_rows(a0, a1, g.scale, dq + qbase, (size_t)g.q_rs, g.Nq);
         const int least = r32 >= len ? 64 : (g.causal ? r32 - start - 4 * hi : -64);   // the first query row that sees this lane's key
         unsigned pp[8], pd[8];
@@ -537,7 +556,7 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
         store_rows(dk0, dk1, g.scale, dk + kbase, (size_t)g.kv_rs, g.Nk);
     }
     // dS^T by distance (a lane each: 31 at most on either side), then by bucket
-    float* block = reinterpret_cast<float*>(&sO[wave][0][0]);   // [32 keys][33], then 64 buckets: 4480 of the wave's 4608 bytes
+    float* block = reinterpret_cast<float*>(&sV[wave][0][0]);   // [32 keys][33], then 64 buckets: 4480 of the wave's 4608 bytes
 #pragma unroll
     for (int r = 0; r < 16; r++) block[((r & 3) + 8 * (r >> 2) + 4 * hi) * 33 + r32] = acc[r];
     wave_order();

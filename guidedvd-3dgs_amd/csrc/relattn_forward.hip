@@ -360,43 +360,43 @@ __global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __re
 
 // ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
 // The whole problem of an item is 3 x 32 x 128 bytes in and 32 x 128 out: memory.  A wave keeps one head (its stride over items is a multiple of H),
-// so its 16 biases a lane stay in registers over all its items; the next item's rows are requested before this one's softmax.
+// so its 16 biases a lane stay in registers over all its items; the next item's rows are requested as soon as this one's registers are free.  Rows are
+// read whole, 8 lanes each, and take their operand forms through one piece of LDS, Q then K then V then the result (LDS operations of a wave keep their order).
 template <typename T>
 __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
                                                    float* __restrict__ lse, int items, int waves)
 {
     typedef typename Tr<T>::vec8 vec8;
-    typedef T T2 __attribute__((ext_vector_type(2)));
-    constexpr int VT_PITCH = 40, O_PITCH = 72;
-    __shared__ __attribute__((aligned(16))) T sVt[4][64][VT_PITCH];
-    __shared__ __attribute__((aligned(16))) T sO[4][32][O_PITCH];
+    constexpr int PITCH = 72;
+    __shared__ __attribute__((aligned(16))) T sRows[4][32][PITCH];
     __shared__ float sB[4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, r32 = lane & 31;
     const int gw = blockIdx.x * 4 + wave;
     if (gw >= waves) return;   // (no barriers below)
     const int h = gw % g.H, step = waves / g.H, nb = items / g.H;
-    const int kp = lane & 15, vo = lane >> 4;
-    const size_t qoff = (size_t)(r32 < g.Nq ? r32 : g.Nq - 1) * (size_t)g.q_rs + (size_t)h * 64 + 8 * hi;
-    vec8 qf[4], kf[4], va[2], vb[2];
-    int len = 0, len_next;
+    const int row = lane >> 3, c8 = 8 * (lane & 7);   // rows 8 i + row
+    T (*rows)[PITCH] = sRows[wave];
+    vec8 rq[4], rk[4], rv[4];
+    int len_next;
     // rows at or behind the length: the last one again; their scores are masked.  (A length of zero: row 0, and the item's result is zeros.)
     auto load = [&](int b) {
         len_next = len_of(g, b);
         const int last = len_next > 0 ? len_next - 1 : 0;
-        const T* qb = q + (size_t)b * g.q_bs + qoff;
-        const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64 + (size_t)(r32 < last ? r32 : last) * (size_t)g.kv_rs + 8 * hi;
-        const T* v0 = v + (size_t)b * g.kv_bs + (size_t)h * 64 + 8 * vo;
-        const size_t off0 = (size_t)(2 * kp < last ? 2 * kp : last) * (size_t)g.kv_rs, off1 = (size_t)(2 * kp + 1 < last ? 2 * kp + 1 : last) * (size_t)g.kv_rs;
+        const T* qb = q + (size_t)b * g.q_bs + (size_t)h * 64 + c8;
+        const size_t kv = (size_t)b * g.kv_bs + (size_t)h * 64 + c8;
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            qf[ks] = *reinterpret_cast<const vec8*>(qb + 16 * ks);
-            kf[ks] = *reinterpret_cast<const vec8*>(kb + 16 * ks);
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + row;
+            rq[i] = *reinterpret_cast<const vec8*>(qb + (size_t)(r < g.Nq ? r : g.Nq - 1) * (size_t)g.q_rs);
+            const size_t off = kv + (size_t)(r < last ? r : last) * (size_t)g.kv_rs;
+            rk[i] = *reinterpret_cast<const vec8*>(k + off);
+            rv[i] = *reinterpret_cast<const vec8*>(v + off);
         }
+    };
+    auto put = [&](const vec8 (&x)[4]) {
 #pragma unroll
-        for (int ps = 0; ps < 2; ps++) {
-            va[ps] = *reinterpret_cast<const vec8*>(v0 + off0 + 32 * ps);
-            vb[ps] = *reinterpret_cast<const vec8*>(v0 + off1 + 32 * ps);
-        }
+        for (int i = 0; i < 4; i++) *reinterpret_cast<vec8*>(&rows[8 * i + row][c8]) = x[i];
+        wave_order();
     };
     f16v bias;
     int biased = 0x7fffffff;   // the start that `bias` is for
@@ -410,29 +410,31 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
     };
     load(gw / g.H);
     for (int b = gw / g.H; b < nb; b += step) {
-        len = len_next;
-        const int start = start_of(g, b);
+        const int len = len_next, start = start_of(g, b);
         if (start != biased) set_bias(start);
+        vec8 qf[4], kf[4];
+        put(rq);
 #pragma unroll
-        for (int ps = 0; ps < 2; ps++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const T2 pr = { va[ps][i], vb[ps][i] };
-                *reinterpret_cast<T2*>(&sVt[wave][(vo + 4 * ps) * 8 + i][2 * kp]) = pr;
-            }
+        for (int ks = 0; ks < 4; ks++) qf[ks] = *reinterpret_cast<const vec8*>(&rows[r32][16 * ks + 8 * hi]);
         wave_order();
+        put(rk);
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) kf[ks] = *reinterpret_cast<const vec8*>(&rows[r32][16 * ks + 8 * hi]);
+        wave_order();
+        put(rv);
+        load(b + step < nb ? b + step : b);
         f16v s = bias;
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) s = Tr<T>::mfma(kf[ks], qf[ks], s);
-        load(b + step < nb ? b + step : b);
         const int seen = (g.causal && start + r32 + 1 < len ? start + r32 + 1 : len) - 4 * hi;
 #pragma unroll
         for (int r = 0; r < 16; r++)
             if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
-        float mt = LOWEST;
+        float mt = max3f(s[0], s[1], s[2]);
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) mt = max3f(mt, s[r] * g.c, s[r + 1] * g.c);
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        for (int r = 3; r < 15; r += 2) mt = max3f(mt, s[r], s[r + 1]);
+        mt = fmaxf(mt, s[15]);
+        mt = fmaxf(fmaxf(mt, __shfl_xor(mt, 32, 64)) * g.c, LOWEST);
         unsigned pk[8];
         float l = 0.f;
 #pragma unroll
@@ -446,11 +448,10 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const vec8 pf = packed_c_to_b_operand<T>(pk, k2);
-            const vec8 a0 = *reinterpret_cast<const vec8*>(&sVt[wave][r32][16 * k2 + 8 * hi]);
-            const vec8 a1 = *reinterpret_cast<const vec8*>(&sVt[wave][32 + r32][16 * k2 + 8 * hi]);
-            o0 = Tr<T>::mfma(a0, pf, o0);
-            o1 = Tr<T>::mfma(a1, pf, o1);
+            o0 = Tr<T>::mfma(transposed_operand(&rows[0][0], PITCH, 16 * k2, 0, lane), pf, o0);
+            o1 = Tr<T>::mfma(transposed_operand(&rows[0][0], PITCH, 16 * k2, 32, lane), pf, o1);
         }
+        wave_order();
         const bool empty = !(l > 0.f) || len == 0;   // (a length of zero: row 0 of V was loaded, whatever it holds)
         if (lse && hi == 0 && r32 < g.Nq) lse[((size_t)b * g.H + h) * g.Nq + r32] = empty ? INFINITY : mt + __builtin_amdgcn_logf(l);
         const float inv = 1.0f / l;
@@ -463,16 +464,16 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
             w1.x = Tr<T>::pack2(o1[4 * rg] * inv, o1[4 * rg + 1] * inv);
             w1.y = Tr<T>::pack2(o1[4 * rg + 2] * inv, o1[4 * rg + 3] * inv);
             if (empty) { w0 = make_uint2(0, 0); w1 = make_uint2(0, 0); }
-            *reinterpret_cast<uint2*>(&sO[wave][r32][d0]) = w0;
-            *reinterpret_cast<uint2*>(&sO[wave][r32][32 + d0]) = w1;
+            *reinterpret_cast<uint2*>(&rows[r32][d0]) = w0;
+            *reinterpret_cast<uint2*>(&rows[r32][32 + d0]) = w1;
         }
         wave_order();
-        T* ob = out + (size_t)b * g.o_bs + (size_t)h * 64 + 8 * (lane & 7);
+        T* ob = out + (size_t)b * g.o_bs + (size_t)h * 64 + c8;
 #pragma unroll
-        for (int ps = 0; ps < 4; ps++) {
-            const int row = (lane >> 3) + 8 * ps;
-            const uint4 w = *reinterpret_cast<const uint4*>(&sO[wave][row][8 * (lane & 7)]);
-            if (row < g.Nq) *reinterpret_cast<uint4*>(ob + (size_t)row * (size_t)g.o_rs) = w;
+        for (int i = 0; i < 4; i++) {
+            const int r = 8 * i + row;
+            const u4 w = *reinterpret_cast<const u4*>(&rows[r][c8]);
+            if (r < g.Nq) __builtin_nontemporal_store(w, reinterpret_cast<u4*>(ob + (size_t)r * (size_t)g.o_rs));
         }
         wave_order();
     }
@@ -608,23 +609,34 @@ enum Form { SHORT, FEW, GENERAL };
 
 struct Plan { Form form; int qb, tiles, parts; };
 
-// Which kernel, and into how many parts the keys are cut.
+// Which kernel, how many query blocks a wave, and into how many parts the keys are cut.
+// General rows: what a choice takes is estimated, in microseconds, and the least is taken.  A workgroup of 128 rows takes 0.95 a tile alone on its CU and 0.745 with
+// others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products); a round of workgroups starts with 4 (bias, first tiles); joining
+// parts takes 4 and 3.3e-5 a row and part.  Measured against it (us): 9216 queries and keys, 5 heads: 128 rows 214, in 2 parts 170; 256 rows 219, in 2 parts
+// 190, in 4 parts 162.  2304, 10 heads: 128 rows 39, 256 rows 58, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 48.5, in 2 parts 55; 256 rows 51.
 Plan plan_of(const Geo& g, int B, int cus)
 {
     const long long bh = (long long)B * g.H;
     if (g.Nq <= 32 && g.Nk <= 32) return { SHORT, 1, 1, 1 };
-    Plan pl;
-    pl.form = g.Nq <= 4 ? FEW : GENERAL;
-    pl.qb = pl.form == GENERAL && g.Nq >= 512 ? 2 : 1;
-    pl.tiles = pl.form == FEW ? 1 : (g.Nq + 128 * pl.qb - 1) / (128 * pl.qb);
-    const long long wgs = bh * pl.tiles, want = (long long)cus * (pl.form == FEW ? 8 : 2);
-    const int least = pl.form == FEW ? 256 : 512;   // keys a part
-    long long parts = wgs < want ? (want + wgs - 1) / wgs : 1;
-    const long long most = (g.Nk + least - 1) / least;
-    if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
-    pl.parts = (int)parts;
-    return pl;
+    if (g.Nq <= 4) {   // few rows: 8 workgroups a CU, at least 256 keys each
+        long long parts = ((long long)cus * 8 + bh - 1) / bh;
+        const long long most = (g.Nk + 255) / 256;
+        if (parts > most) parts = most;
+        return { FEW, 1, 1, (int)(parts < 64 ? parts : 64) };
+    }
+    Plan best = { GENERAL, 1, 1, 1 };
+    double least = 1e30;
+    const int tiles = (g.Nk + KV_TILE - 1) / KV_TILE;
+    for (int qb = 1; qb <= 2; qb++) {
+        const int rows = 128 * qb, qtiles = (g.Nq + rows - 1) / rows;
+        for (int parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= tiles); parts++) {
+            const double load = (double)bh * qtiles * parts / cus, rounds = load <= 1.0 ? 1.0 : (load < 8.0 ? __builtin_ceil(load) : load);
+            const double a_tile = rounds == 1.0 ? (qb == 2 ? 1.5 : 0.95) : rounds * (qb == 2 ? 1.3 : 0.745);
+            const double t = 4.0 * rounds + (tiles + parts - 1) / parts * a_tile + (parts > 1 ? 4.0 + 3.3e-5 * (double)bh * g.Nq * parts : 0.0);
+            if (t < least) { least = t; best = { GENERAL, qb, qtiles, parts }; }
+        }
+    }
+    return best;
 }
 
 size_t part_rows(const Geo& g, int B, const Plan& pl) { return (size_t)pl.parts * B * g.H * g.Nq; }
@@ -646,8 +658,8 @@ int launch_fwd(const Geo& g, int B, const void* q, const void* k, const void* v,
     }
     const size_t lds = sizeof(float) * bias_len(g.reach);
     if (pl.form == SHORT) {
-        // as many waves as stay resident (4 workgroups a CU by LDS), a multiple of the heads
-        long long waves = (long long)cus * 16;
+        // 8 waves a CU, a multiple of the heads (46080 items of 25 frames: 118.7 us; with 4 115.8, 12 127, 16 123; 11200 items with the backward: 101, 4 110, 16 102)
+        long long waves = (long long)cus * 8;
         if (waves > BH) waves = BH;
         waves = waves >= g.H ? waves / g.H * g.H : g.H;
         hipLaunchKernelGGL(k_rel_short<T>, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, BH, (int)waves);
