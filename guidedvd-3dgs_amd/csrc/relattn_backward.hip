@@ -110,7 +110,9 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
         for (int j = 0; j < 8; j++) Dl = fmaf((float)x[j], (float)gf[ks][j], Dl);
     }
     Dl += __shfl_xor(Dl, 32, 64);
-    f16v dq0 = {}, dq1 = {};
+    f16v dq0 = {}, dq1 = {}, minus_delta;   // (dP's accumulators start from -delta: dS = P o what comes out)
+#pragma unroll
+    for (int r = 0; r < 16; r++) minus_delta[r] = -Dl;
     float off = 0.f;   // this lane's part of the row's sum of dS
 
     vec8 rk = {}, rv = {};
@@ -140,7 +142,7 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
             }
         }
         const int k0 = kt + half;   // the wave's 32 keys
-        f16v s = {}, dp = {};
+        f16v s = {}, dp = minus_delta;
         float shift = -L;           // weights are exp2(s c + shift): a single bias of the block goes here
         const bool past = k0 + 31 - first <= -g.reach, ahead = k0 - first - 31 >= g.reach;
         if (past || ahead) shift += past ? far_past : far_ahead;
@@ -163,8 +165,8 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
         unsigned pd[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float d0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)) * (dp[2 * j] - Dl);
-            const float d1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift)) * (dp[2 * j + 1] - Dl);
+            const float d0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)) * dp[2 * j];
+            const float d1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift)) * dp[2 * j + 1];
             off += d0 + d1;
             pd[j] = Tr<T>::pack2(d0, d1);
         }
@@ -200,7 +202,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
 {
     typedef typename Tr<T>::vec8 vec8;
     __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: Q, b: dO
-    __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // lse and delta of a tile's rows
+    __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // -lse / c and -delta of a tile's rows: where the accumulators of S and dP start
     __shared__ float sFar[8][2];
     __shared__ float sSkew[8][16 * 48];
     extern __shared__ __attribute__((aligned(16))) float sBias[];   // the bias, then 8 arrays of sums by distance
@@ -216,6 +218,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     const T* gb = d_o + (size_t)b * g.o_bs + (size_t)h * 64;
     const size_t kvoff = (size_t)b * g.kv_bs + (size_t)h * 64;
     const float* row_b = (wave == 0 ? lse : delta) + (size_t)bh * g.Nq;   // what waves 0 and 1 bring
+    const float row_factor = wave == 0 ? -1.0f / g.c : -1.0f;
 
     const int k0 = tile_y * 128, kw = k0 + (wave & 3) * 32, key = kw + col;
     const bool there = key < len;
@@ -245,7 +248,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     auto commit = [&](int qt, int buf) {
         tile_commit(rq, qt, g.Nq, tid, tiles.a[buf]);
         tile_commit(rg, qt, g.Nq, tid, tiles.b[buf]);
-        if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? rr : (wave == 0 ? INFINITY : 0.f);   // rows past the end weigh 0
+        if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? rr * row_factor : (wave == 0 ? -INFINITY : 0.f);   // rows past the end weigh 0
     };
     if (q_lo < g.Nq) prefetch(q_lo);
     for (int e = tid; e < 8 * blen; e += 512) sBias[blen + e] = 0.f;
@@ -265,13 +268,20 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         }
         const int first = start + qt + half;   // position of the block's first query
         const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
-        f16v s = {}, dp = {};
-        float shift = 0.f;
+        f16v s, dp;
+#pragma unroll
+        for (int g4 = 0; g4 < 4; g4++) {   // rows 8 g4 + 4 hi + {0 .. 3}
+            const f4v L = *reinterpret_cast<const f4v*>(&sRow[buf][0][half + 8 * g4 + 4 * hi]);
+            const f4v D = *reinterpret_cast<const f4v*>(&sRow[buf][1][half + 8 * g4 + 4 * hi]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) { s[4 * g4 + j] = L[j]; dp[4 * g4 + j] = D[j]; }
+        }
+        float shift = 0.f;   // weights are exp2(s c + shift): a single bias of the block goes here
         const int e0 = key - first - 4 * hi + span - 27;   // row r of the block: e0 + 27 - (r & 3) - 8 (r >> 2)
         if (past || ahead) shift = past ? far_past : far_ahead;
         else {
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = sBias[e0 + (27 - (r & 3) - 8 * (r >> 2))];
+            for (int r = 0; r < 16; r++) s[r] += sBias[e0 + (27 - (r & 3) - 8 * (r >> 2))];
         }
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
@@ -287,19 +297,12 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         float ds[16];
         unsigned pp[8], pd[8];
 #pragma unroll
-        for (int g4 = 0; g4 < 4; g4++) {   // rows 8 g4 + 4 hi + {0 .. 3}
-            const f4v L = *reinterpret_cast<const f4v*>(&sRow[buf][0][half + 8 * g4 + 4 * hi]);
-            const f4v D = *reinterpret_cast<const f4v*>(&sRow[buf][1][half + 8 * g4 + 4 * hi]);
-            float p[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                p[j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g4 + j], g.c, shift - L[j]));
-                ds[4 * g4 + j] = p[j] * (dp[4 * g4 + j] - D[j]);
-            }
-            pp[2 * g4] = Tr<T>::pack2(p[0], p[1]);
-            pp[2 * g4 + 1] = Tr<T>::pack2(p[2], p[3]);
-            pd[2 * g4] = Tr<T>::pack2(ds[4 * g4], ds[4 * g4 + 1]);
-            pd[2 * g4 + 1] = Tr<T>::pack2(ds[4 * g4 + 2], ds[4 * g4 + 3]);
+        for (int j = 0; j < 8; j++) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift));
+            ds[2 * j] = p0 * dp[2 * j];
+            ds[2 * j + 1] = p1 * dp[2 * j + 1];
+            pp[j] = Tr<T>::pack2(p0, p1);
+            pd[j] = Tr<T>::pack2(ds[2 * j], ds[2 * j + 1]);
         }
         if (past || ahead) {
             float x = 0.f;

@@ -481,6 +481,8 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
 
 // ---- few queries, many keys ----------------------------------------------------------------------------------------------------
 // 8 lanes hold a key's 64 channels, a wave 8 keys at once, 4 of those in flight; every lane group keeps its own running maximum and sum, joined at the end.
+// 16 x 10 rows against caches of 8192 (half full on average): 41 us with the join, 4.3 TB/s; with ordinary loads 45, with an item's parts on one XCD 3 more, with
+// 8 workgroups a CU 41 (and 64 x 20 rows against 1000: 39 against 36), with 8 keys a lane group in flight 63.
 template <typename T, int NQ>
 __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
                                                  float* __restrict__ lse, float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
@@ -490,8 +492,7 @@ __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restric
     __shared__ float sO[4][NQ][64];
     __shared__ float sM[4][NQ], sL[4][NQ];
     extern __shared__ __attribute__((aligned(16))) float sBias[];
-    int bh, part;
-    xcd_item_tile(bh, part);
+    const int bh = blockIdx.x, part = blockIdx.y;   // the heads of a key lie next to each other: their workgroups run at once
     const int b = bh / g.H, h = bh - b * g.H;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 3, sub = lane & 7;
     const int start = start_of(g, b), len = len_of(g, b);
@@ -506,8 +507,8 @@ __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restric
         for (int u = 0; u < U; u++) {
             const int j = base + 8 * u + grp;
             const size_t off = (size_t)(j < k_hi ? j : k_hi - 1) * (size_t)g.kv_rs;
-            kf[u] = *reinterpret_cast<const vec8*>(kb + off);
-            vf[u] = *reinterpret_cast<const vec8*>(vb + off);
+            kf[u] = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(kb + off));
+            vf[u] = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(vb + off));
         }
     };
     const int base0 = k_lo + wave * 32;
@@ -611,15 +612,15 @@ struct Plan { Form form; int qb, tiles, parts; };
 
 // Which kernel, how many query blocks a wave, and into how many parts the keys are cut.
 // General rows: what a choice takes is estimated, in microseconds, and the least is taken.  A workgroup of 128 rows takes 0.95 a tile alone on its CU and 0.745 with
-// others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products); a round of workgroups starts with 4 (bias, first tiles); joining
-// parts takes 4 and 3.3e-5 a row and part.  Measured against it (us): 9216 queries and keys, 5 heads: 128 rows 214, in 2 parts 170; 256 rows 219, in 2 parts
+// others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products); a round of workgroups starts with 4 (bias, first tiles); parts
+// take 8 (their stores, the join's launch) and 3.3e-5 a row and part.  Measured against it (us): 9216 queries and keys, 5 heads: 128 rows 214, in 2 parts 170; 256 rows 219, in 2 parts
 // 190, in 4 parts 162.  2304, 10 heads: 128 rows 39, 256 rows 58, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 48.5, in 2 parts 55; 256 rows 51.
 Plan plan_of(const Geo& g, int B, int cus)
 {
     const long long bh = (long long)B * g.H;
     if (g.Nq <= 32 && g.Nk <= 32) return { SHORT, 1, 1, 1 };
-    if (g.Nq <= 4) {   // few rows: 8 workgroups a CU, at least 256 keys each
-        long long parts = ((long long)cus * 8 + bh - 1) / bh;
+    if (g.Nq <= 4) {   // few rows: 4 workgroups a CU, at least 256 keys each
+        long long parts = ((long long)cus * 4 + bh - 1) / bh;
         const long long most = (g.Nk + 255) / 256;
         if (parts > most) parts = most;
         return { FEW, 1, 1, (int)(parts < 64 ? parts : 64) };
@@ -632,7 +633,7 @@ Plan plan_of(const Geo& g, int B, int cus)
         for (int parts = 1; parts <= 64 && (parts == 1 || 2 * parts <= tiles); parts++) {
             const double load = (double)bh * qtiles * parts / cus, rounds = load <= 1.0 ? 1.0 : (load < 8.0 ? __builtin_ceil(load) : load);
             const double a_tile = rounds == 1.0 ? (qb == 2 ? 1.5 : 0.95) : rounds * (qb == 2 ? 1.3 : 0.745);
-            const double t = 4.0 * rounds + (tiles + parts - 1) / parts * a_tile + (parts > 1 ? 4.0 + 3.3e-5 * (double)bh * g.Nq * parts : 0.0);
+            const double t = 4.0 * rounds + (tiles + parts - 1) / parts * a_tile + (parts > 1 ? 8.0 + 3.3e-5 * (double)bh * g.Nq * parts : 0.0);
             if (t < least) { least = t; best = { GENERAL, qb, qtiles, parts }; }
         }
     }
