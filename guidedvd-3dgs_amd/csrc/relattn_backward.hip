@@ -4,9 +4,10 @@
 //     dQ = scale dS K,  dK = scale dS^T Q,  dT[b, h] = sum of dS_ij over the (i, j) whose distance lies in bucket b
 //
 // General rows, kernels in turn, no sum whose order could change:
-//   k_rel_dq      a wave = 32 queries; delta from dO . O: O was rounded, and so were the P that made it, so this delta is 2^-9 off (bf16) -- enough for 16-bit
-//                 gradients, not for a table's gradient in 32 bits: its sums cancel (a row's dS sums to 0).  Walks the keys, and also sums each row's dS, which is
-//                 exactly what delta was off by: the delta that it leaves for k_rel_dkv is right
+//   k_rel_dq      a wave = 32 queries; walks the keys with delta from dO . O.  O was rounded, and so were the P that made it, so this delta is 2^-9 |dO| |O| off
+//                 (bf16), which is much where V has a mean (dS is a difference then) and for a table's gradient in 32 bits (its sums cancel: a row's dS
+//                 sums to 0).  But a row's dS as formed sums to exactly what delta was off by, so dQ = dS K - (that sum) P K, one more product on K's
+//                 fragments, and the delta that the kernel leaves for k_rel_dkv is right.  (V = noise + 3, bf16: dQ 2.1 % off without, 0.24 % with)
 //   k_rel_dkv     a wave = 32 keys; walks the queries; dS of the table from the corrected delta: by distance into an array of the wave's own in LDS, blocks beyond
 //                 the last border into one register; at the end distances are summed into buckets, one row of partial sums a workgroup
 //   k_rel_table   sums the partial rows, 64 bits
@@ -77,7 +78,7 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
 {
     typedef typename Tr<T>::vec8 vec8;
     __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: K, b: V
-    __shared__ float sOff[4][32];
+    __shared__ float sOff[8][32];
     extern __shared__ __attribute__((aligned(16))) float sBias[];
 
     int bh, tile_y;
@@ -110,7 +111,7 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
         for (int j = 0; j < 8; j++) Dl = fmaf((float)x[j], (float)gf[ks][j], Dl);
     }
     Dl += __shfl_xor(Dl, 32, 64);
-    f16v dq0 = {}, dq1 = {}, minus_delta;   // (dP's accumulators start from -delta: dS = P o what comes out)
+    f16v dq0 = {}, dq1 = {}, pk0 = {}, pk1 = {}, minus_delta;   // (dP's accumulators start from -delta: dS = P o what comes out)
 #pragma unroll
     for (int r = 0; r < 16; r++) minus_delta[r] = -Dl;
     float off = 0.f;   // this lane's part of the row's sum of dS
@@ -162,34 +163,41 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
             for (int r = 0; r < 16; r++)
                 if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
         }
-        unsigned pd[8];
+        unsigned pp[8], pd[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float d0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)) * dp[2 * j];
-            const float d1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift)) * dp[2 * j + 1];
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift));
+            const float d0 = p0 * dp[2 * j], d1 = p1 * dp[2 * j + 1];
             off += d0 + d1;
+            pp[j] = Tr<T>::pack2(p0, p1);
             pd[j] = Tr<T>::pack2(d0, d1);
         }
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 df = packed_c_to_b_operand<T>(pd, k2);
-            dq0 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), df, dq0);
-            dq1 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), df, dq1);
+            const vec8 df = packed_c_to_b_operand<T>(pd, k2), pf = packed_c_to_b_operand<T>(pp, k2);
+            const vec8 a0 = transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane);
+            const vec8 a1 = transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane);
+            dq0 = Tr<T>::mfma(a0, df, dq0);
+            dq1 = Tr<T>::mfma(a1, df, dq1);
+            pk0 = Tr<T>::mfma(a0, pf, pk0);
+            pk1 = Tr<T>::mfma(a1, pf, pk1);
         }
         __syncthreads();
     }
     off += __shfl_xor(off, 32, 64);
+    if (hi == 0) sOff[wave][col] = off;
+    __syncthreads();
+    off = sOff[wave & 3][col] + sOff[(wave & 3) + 4][col];
+#pragma unroll
+    for (int r = 0; r < 16; r++) { dq0[r] = fmaf(-off, pk0[r], dq0[r]); dq1[r] = fmaf(-off, pk1[r], dq1[r]); }
     float* at = reinterpret_cast<float*>(&tiles);
-    if (wave >= 4) {
-        hand_over(at, wave, lane, dq0, dq1);
-        if (hi == 0) sOff[wave & 3][col] = off;
-    }
+    if (wave >= 4) hand_over(at, wave, lane, dq0, dq1);
     __syncthreads();
     if (wave < 4) {
         take_over(at, wave, lane, dq0, dq1);
         if (valid) {
             store_row<T>(dq + qrow, dq0, dq1, g.scale, hi);
-            if (hi == 0) delta[(size_t)bh * g.Nq + query] = Dl + off + sOff[wave][col];   // sum_j P dP = delta sum_j P + sum_j dS, and the weights sum to 1
+            if (hi == 0) delta[(size_t)bh * g.Nq + query] = Dl + off;   // sum_j P dP = delta sum_j P + sum_j dS, and the weights sum to 1
         }
     }
 }
