@@ -236,9 +236,10 @@ class RasterTrainer:
     0.8 L1 + 0.2 (1 - SSIM), backward) + one pseudo view once generated frames exist (L1 against the frame, :357-372), one Adam
     step over all Gaussian parameters -- plus the 25 no-grad guidance renders of a diffusion run (:500-527) and the pseudo-view
     stack (:612-636).  The reference's random picks are replaced by deterministic ones (train view it % n, pseudo view by a
-    fixed stride) so that runs are comparable across layouts."""
+    fixed stride) so that runs are comparable across layouts.
+    optimizer: "adam" (torch.optim.Adam), or the same rule as one launch, "fused" (fused_optim.FusedAdamW) or "fused8" (its moments in 8 bits)."""
 
-    def __init__(self, scene, traj_cameras, device, roles=None, cond_hw=(320, 448), lr=1e-4, lambda_dssim=0.2):
+    def __init__(self, scene, traj_cameras, device, roles=None, cond_hw=(320, 448), lr=1e-4, lambda_dssim=0.2, optimizer="adam"):
         import numpy as np
         from diff_gaussian_rasterization import GaussianRasterizationSettings
         self.device, self.roles = torch.device(device), roles
@@ -262,9 +263,18 @@ class RasterTrainer:
         self.gts = [torch.rand((3, self.H, self.W), device=self.device, generator=gen) for _ in self.train_cams]
         self.cond_hw = tuple(cond_hw)
         self.lambda_dssim = lambda_dssim
-        self.opt = torch.optim.Adam(list(self.params.values()), lr=lr, eps=1e-15)
+        self.opt = self._optimizer(optimizer, list(self.params.values()), lr)
         self.pseudo = []          # [(trajectory camera index, pseudo ground truth [3,H,W])]
         self.runs_consumed = []
+
+    @staticmethod
+    def _optimizer(kind, params, lr):
+        if kind == "adam":
+            return torch.optim.Adam(params, lr=lr, eps=1e-15)
+        from fused_optim import FusedAdamW
+        if kind not in ("fused", "fused8"):
+            raise ValueError(f"RasterTrainer: optimizer is 'adam', 'fused' or 'fused8', not {kind!r}")
+        return FusedAdamW(params, lr=lr, eps=1e-15, weight_decay=0.0, state_bits=32 if kind == "fused" else 8)
 
     def spec(self):
         return PacketSpec(len(self.traj_cams), self.H, self.W, *self.cond_hw)

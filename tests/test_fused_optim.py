@@ -482,3 +482,36 @@ def test_runs_on_the_current_stream():
     z = torch.zeros(old.shape)
     rp, _, _, ep, _, _ = reference(old, gs[0][0], z, z, 1, 1e-2, 0.9, 0.999, 1e-8, 0.0)
     assert bool(((p.detach().double().cpu() - rp).abs() <= ep).all())
+
+
+# ---- in the trainer --------------------------------------------------------------------------------------------------------------
+def test_the_trainer_names_its_optimizers():
+    import guided_schedule as gs
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    a, f, e = (gs.RasterTrainer._optimizer(k, p, 1e-4) for k in ("adam", "fused", "fused8"))
+    assert type(a) is torch.optim.Adam and type(f) is FusedAdamW and f.param_groups[0]["state_bits"] == 32 and e.param_groups[0]["state_bits"] == 8
+    for o in (a, f, e):
+        assert o.param_groups[0]["eps"] == 1e-15 and o.param_groups[0]["weight_decay"] == 0
+    with pytest.raises(ValueError, match="optimizer"):
+        gs.RasterTrainer._optimizer("sgd", p, 1e-4)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fused", "fused8"])
+def test_training_gaussians(kind):
+    """One step of the raster trainer from the same start as torch's Adam: the gradients are the same bits, so parameters are equal to the update's float32 (the
+    first step is lr times the gradient's sign, 12 U off at most, and sums with p are rounded); then it goes on."""
+    import guided_schedule as gs
+    import synthetic as syn
+    sc = syn.scene_c1()
+    ref, got = (gs.RasterTrainer(sc, sc["cameras"], DEV, lr=1e-3, optimizer=k) for k in ("adam", kind))
+    ref.train_step(0)
+    got.train_step(0)
+    for n, x in ref.state().items():
+        y = got.state()[n]
+        assert bool(((x - y).abs() <= 4 * U * x.abs() + 16 * U * 1e-3).all()), n
+    before = got.state()
+    for it in range(1, 6):
+        got.train_step(it)
+    after = got.state()
+    assert all(bool(torch.isfinite(x).all()) for x in after.values()) and not torch.equal(before["means3D"], after["means3D"])

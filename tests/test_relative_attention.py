@@ -88,8 +88,9 @@ def formula(q, k, v, table, H, g=None, *, max_distance=128, bidirectional=True, 
     dp = G @ V.transpose(-1, -2)
     delta = (p * dp).sum(-1, keepdim=True)
     ds = p * (dp - delta)
+    # dQ first forms dS with delta from the rounded output, off by up to e_delta, and takes (that) P K off again: only the roundings of both see it
     e_delta = (G.abs() * e_o).sum(-1, keepdim=True) + d32 * (p * dp.abs()).sum(-1, keepdim=True)
-    e_ds = u * ds.abs() + p * e_delta + 2 * d32 * p * (dp.abs() + delta.abs()) + small
+    e_ds = u * (ds.abs() + 2 * p * e_delta) + 2 * d32 * p * (dp.abs() + delta.abs()) + small
     dq, dk = ds @ K * scale, ds.transpose(-1, -2) @ Q * scale
     res |= dict(dq=rows_of(dq, fm), dk=rows_of(dk, fm), dv=rows_of(dv, fm))
     err |= dict(dq=rows_of(e_ds @ K.abs() * scale + u * dq.abs() + small, fm), dk=rows_of(e_ds.transpose(-1, -2) @ Q.abs() * scale + u * dk.abs() + small, fm),
@@ -295,6 +296,20 @@ def test_a_table_of_32_bits_has_a_gradient_of_32_bits():
         t.requires_grad_(True)
         (dt,) = torch.autograd.grad(ops.relative_bias_attention(q, k, v, t, shape[1], **kw), t, g)
         assert float((dt.double() - want["dtable"]).norm() / want["dtable"].norm()) < 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_with_a_mean(dtype):
+    """dS is a difference of numbers of the mean's size.  Two roundings to the type lie between exact sums and each gradient (dS or P as a factor, the result):
+    2 x eps / 2 of the norm, where a delta from the rounded output alone would leave about ten times that."""
+    q, k, v, t, g = inputs(1, 3, 300, 300, dtype, seed=3)
+    k, v = (k.float() + 0.5).to(dtype), (v.float() + 3.0).to(dtype)
+    want, _ = formula(q, k, v, t, 3, g)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, t)]
+    got = dict(zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(ops.relative_bias_attention(*leaves, 3), leaves, g)))
+    for n in ("dq", "dk", "dv"):
+        assert float((got[n].double() - want[n]).norm() / want[n].norm()) < torch.finfo(dtype).eps, n
 
 
 # ---- masks -----------------------------------------------------------------------------------------------------------------------
