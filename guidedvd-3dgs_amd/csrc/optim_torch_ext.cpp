@@ -9,8 +9,8 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <cmath>
-#include <unordered_set>
 
 #include "../../include/gvd_optim.h"
 
@@ -74,7 +74,7 @@ void adamw_step(const std::vector<at::Tensor>& flat, const std::vector<double>& 
 
     std::vector<gvd_adamw_tensor> table(n);
     std::vector<at::Tensor> grads(n);   // (keeps copies made here alive)
-    std::unordered_set<const void*> seen;
+    std::vector<std::pair<const char*, const char*>> spans(n);
     for (size_t i = 0; i < n; i++) {    // everything is checked before anything is counted or launched
         const at::Tensor &p = flat[i * per], &g = flat[i * per + 1], &step = flat[i * per + 2], &m = flat[i * per + 3], &v = flat[i * per + 4];
         TORCH_CHECK(g.layout() == at::kStrided, "FusedAdamW: sparse gradients are not supported");
@@ -93,7 +93,7 @@ void adamw_step(const std::vector<at::Tensor>& flat, const std::vector<double>& 
             t.exp_avg_scale = flat[i * per + 5].data_ptr<float>();
             t.exp_avg_sq_scale = flat[i * per + 6].data_ptr<float>();
         }
-        TORCH_CHECK(p.numel() == 0 || seen.insert(p.data_ptr()).second, "FusedAdamW: two parameters share their memory");
+        spans[i] = {(const char*)p.data_ptr(), (const char*)p.data_ptr() + p.nbytes()};
         grads[i] = same_order(p, g) ? g : at::empty_like(p).copy_(g);
         t.param = p.data_ptr();
         t.grad = grads[i].data_ptr();
@@ -102,6 +102,9 @@ void adamw_step(const std::vector<at::Tensor>& flat, const std::vector<double>& 
         t.n = p.numel();
         if (!lr_at.empty() && lr_at[i]) TORCH_CHECK(lr_at[i]->device() == device, "FusedAdamW: lr is on another device than its parameters");
     }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < n; i++)
+        TORCH_CHECK(spans[i].first >= spans[i - 1].second || spans[i - 1].first == spans[i - 1].second, "FusedAdamW: two parameters share memory");
     void* stream = (void*)c10::hip::getCurrentHIPStream(device.index()).stream();
     at::Tensor scalars;
     if (capturable) {

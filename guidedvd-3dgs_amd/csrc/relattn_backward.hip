@@ -617,7 +617,8 @@ int launch_bwd(const Geo& g, int B, const void* q, const void* k, const void* v,
     } else {
         tiles = (g.Nk + 127) / 128;
         const int qtiles = (g.Nq + 127) / 128;
-        if (BH > (1 << 23) || tiles > 65535 || qtiles > 65535 || (long long)B * tiles > 0x7fffffffLL) return fail(-1, "gvd_relattn_bwd: too many workgroups");
+        if (BH > (1 << 22) || tiles > 65535 || qtiles > 65535 || (long long)BH * (tiles > qtiles ? tiles : qtiles) > 0x7fffffffLL)
+            return fail(-1, "gvd_relattn_bwd: too many workgroups");
         count = B * tiles;
         const size_t lds = sizeof(float) * bias_len(g.reach);
         hipLaunchKernelGGL(k_rel_dq<T>, dim3((unsigned)BH, (unsigned)qtiles), dim3(512), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (const T*)out,

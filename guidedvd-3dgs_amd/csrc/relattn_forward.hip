@@ -648,7 +648,8 @@ int launch_fwd(const Geo& g, int B, const void* q, const void* k, const void* v,
     const int cus = compute_units();
     const Plan pl = plan_of(g, B, cus);
     const int BH = B * g.H;
-    if (pl.form != SHORT && (BH > (1 << 23) || (long long)pl.tiles * pl.parts > 65535)) return fail(-1, "gvd_relattn_fwd: too many workgroups");
+    if (pl.form != SHORT && (BH > (1 << 23) || (long long)pl.tiles * pl.parts > 65535 || (long long)BH * pl.tiles * pl.parts > 0x7fffffffLL))
+        return fail(-1, "gvd_relattn_fwd: too many workgroups");
     float* po = nullptr;
     float2* ml = nullptr;
     if (pl.parts > 1) {

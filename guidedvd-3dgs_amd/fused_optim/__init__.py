@@ -209,6 +209,9 @@ class FusedAdamW(torch.optim.Optimizer):
         for g in self.param_groups:
             for k, d in self.defaults.items():      # groups saved by torch.optim.Adam / AdamW lack this optimizer's own entries
                 g.setdefault(k, d)
+            if g.get("amsgrad") or g.get("maximize") or g["weight_decay"] and g.get("decoupled_weight_decay") is False:
+                raise ValueError("FusedAdamW: the saved optimizer has another rule (amsgrad, maximize, or weight decay that is not decoupled)")
+            self._check_group(g)
         params = [(p, g) for g in self.param_groups for p in g["params"]]
         for i, (p, g) in zip(saved, params):
             src = state_dict["state"].get(i)
@@ -218,6 +221,8 @@ class FusedAdamW(torch.optim.Optimizer):
             for k, v in src.items():
                 if torch.is_tensor(v) and k != "step":
                     st[k] = v.detach().to(device=p.device, copy=True)
+                    if v.dtype == torch.float32 and v.shape == p.shape and st[k].stride() != p.stride():
+                        st[k] = _like(p, torch.float32).copy_(v)
             step = torch.as_tensor(src["step"], dtype=torch.float32).detach()
             st["step"] = step.to(device=p.device if g["capturable"] else "cpu", copy=True).reshape(())
             self._check_state(p, st, g["state_bits"])

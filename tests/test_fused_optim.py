@@ -83,6 +83,8 @@ def test_c_entry_checks_its_arguments_before_any_launch():
         assert L.gvd_adamw_step(*args, None, None) == -1 and word in L.gvd_optim_last_error(), (args, L.gvd_optim_last_error())
     negative = TENSOR.pack(0, 0, 0, 0, 0, 0, -1, 0.1, 1.0, 1.0, 0)
     assert L.gvd_adamw_step(negative, 1, 0, 32, 0.9, 0.999, 1e-8, None, None) == -1 and b"size" in L.gvd_optim_last_error()
+    huge = TENSOR.pack(16, 16, 16, 16, 0, 0, 2 ** 34 + 1, 0.1, 1.0, 1.0, 0)
+    assert L.gvd_adamw_step(huge, 1, 0, 32, 0.9, 0.999, 1e-8, None, None) == -1 and b"size" in L.gvd_optim_last_error()
     empty = TENSOR.pack(0, 0, 0, 0, 0, 0, 0, 0.1, 1.0, 1.0, 0)
     assert L.gvd_adamw_step(empty, 1, 0, 32, 0.9, 0.999, 1e-8, None, None) == 0      # nothing to do, nothing launched
     assert L.gvd_adamw_scalars(None, None, None, None, None, 1, ctypes.c_double(0.9), ctypes.c_double(0.999), 0, None, None) == -1
@@ -152,6 +154,23 @@ def test_moments_and_state_dicts_round_trip(bits):
     sd["param_groups"][0]["state_bits"] = 40 - bits
     with pytest.raises(RuntimeError, match="does not fit"):
         wrong.load_state_dict(sd)
+
+
+def test_refuses_the_state_of_another_rule():
+    p = torch.nn.Parameter(torch.randn(5, 3))
+    for other in (torch.optim.Adam([p], amsgrad=True), torch.optim.Adam([p], maximize=True), torch.optim.Adam([p], weight_decay=0.1)):
+        with pytest.raises(ValueError, match="rule"):
+            FusedAdamW([p]).load_state_dict(other.state_dict())
+    FusedAdamW([p]).load_state_dict(torch.optim.AdamW([p], weight_decay=0.1).state_dict())
+
+
+def test_state_is_loaded_into_the_parameters_memory_order():
+    p, q = torch.nn.Parameter(torch.randn(5, 3)), torch.nn.Parameter(torch.randn(3, 5).t())
+    a, b = FusedAdamW([p]), FusedAdamW([q])
+    m, v = torch.randn(5, 3), torch.rand(5, 3)
+    a.set_moments(p, m, v, 3)
+    b.load_state_dict(a.state_dict())
+    assert b.state[q]["exp_avg"].stride() == q.stride() and torch.equal(b.state[q]["exp_avg"], m) and torch.equal(b.state[q]["exp_avg_sq"], v)
 
 
 def test_loads_the_state_of_torchs_adam():
@@ -303,10 +322,38 @@ def test_refusals_on_the_device():
     a.grad, b.grad = torch.zeros(4, device=DEV), torch.zeros(4, device=DEV)
     with pytest.raises(RuntimeError, match="share"):
         FusedAdamW([a, b]).step()
+    b = torch.nn.Parameter(base[2:6])                # overlapping in part
+    b.grad = torch.zeros(4, device=DEV)
+    with pytest.raises(RuntimeError, match="share"):
+        FusedAdamW([b, a]).step()
+    b = torch.nn.Parameter(base[4:])                 # side by side
+    b.grad = torch.ones(4, device=DEV)
+    FusedAdamW([b, a], lr=0.5).step()
+    assert bool((base[:4] == 0).all()) and bool((base[4:] < 0).all())
     s = torch.nn.Parameter(torch.zeros(4, 4, device=DEV))
     s.grad = torch.zeros(4, 4, device=DEV).to_sparse()
     with pytest.raises(RuntimeError, match="sparse"):
         FusedAdamW([s]).step()
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """2^31 elements and some: the last ones as in a small tensor, the first untouched by them."""
+    n, tail = 2 ** 31 + 2048 + 5, 5000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device=DEV))
+    p.grad = torch.zeros_like(p)
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    small = torch.nn.Parameter(torch.randn(tail, device=DEV, generator=gen).bfloat16())
+    small.grad = torch.randn(tail, device=DEV, generator=gen).bfloat16()
+    with torch.no_grad():
+        p[-tail:] = small
+        p.grad[-tail:] = small.grad
+    big, ref = FusedAdamW([p], lr=1e-2), FusedAdamW([small], lr=1e-2)
+    big.step()
+    ref.step()
+    assert torch.equal(p[-tail:], small) and not bool(p[:tail].any())
+    assert torch.equal(big.state[p]["exp_avg"][-tail:], ref.state[small]["exp_avg"])
+    assert int(big.state[p]["exp_avg_sq"].count_nonzero()) == int(ref.state[small]["exp_avg_sq"].count_nonzero())   # nothing written elsewhere
 
 
 # ---- 8-bit moments ----------------------------------------------------------------------------------------------------------------

@@ -181,6 +181,11 @@ def test_c_entry_checks_its_arguments_before_any_launch():
         assert L.gvd_relattn_fwd_workspace(ctypes.byref(bad)) == -1 and word in L.gvd_relattn_last_error(), (kw, L.gvd_relattn_last_error())
         assert L.gvd_relattn_bwd_workspace(ctypes.byref(bad)) == -1
         assert L.gvd_relattn_fwd(ctypes.byref(bad), *[ctypes.c_void_p(16)] * 8) == -1 and L.gvd_relattn_bwd(ctypes.byref(bad), *[ctypes.c_void_p(16)] * 13) == -1
+    long, _ = problem(Nq=600, Nk=3000)            # its keys are walked in parts, which need room
+    assert L.gvd_relattn_fwd_workspace(ctypes.byref(long)) > 0
+    assert L.gvd_relattn_fwd(ctypes.byref(long), *[ctypes.c_void_p(16)] * 5, None, None, None) == -1 and b"workspace" in L.gvd_relattn_last_error()
+    many, _ = problem(B=1 << 21, H=8, Nq=1, Nk=40)
+    assert L.gvd_relattn_fwd(ctypes.byref(many), *[ctypes.c_void_p(16)] * 8) == -1 and b"workgroups" in L.gvd_relattn_last_error()
     starts, _ = problem(q_starts=16)
     assert L.gvd_relattn_bwd(ctypes.byref(starts), *[ctypes.c_void_p(16)] * 13) == -1 and b"q_start" in L.gvd_relattn_last_error()
     shared, _ = problem(B=2, kv_bs=0)
