@@ -19,18 +19,27 @@ using namespace gvdr;
 
 namespace {
 
-// A tile of 64 rows x 64 channels through 512 lanes, 16 bytes each: eight lanes a row.  Rows at or behind n_rows: the last one again (n_rows >= 1), and zeros in LDS.
-template <typename T>
-__device__ __forceinline__ typename Tr<T>::vec8 tile_load(const T* __restrict__ src, size_t rs, int row0, int n_rows, int tid)
-{
-    const int row = row0 + (tid >> 3);
-    return *reinterpret_cast<const typename Tr<T>::vec8*>(src + (size_t)(row < n_rows ? row : n_rows - 1) * rs + (tid & 7) * 8);
-}
+// Tiles of 64 rows x 64 channels in turn, through 512 lanes, 16 bytes each: eight lanes a row.  Rows at or behind n_rows: the last one again (n_rows >= 1), and zeros
+// in LDS.  The address moves along: a row's number times the stride, in 64 bits, would take the vector unit as long as 40 additions a lane and tile.
+template <typename T> struct TileRows {
+    const T *at, *last;
+    size_t step;
+    int row, n_rows;
+    __device__ __forceinline__ TileRows(const T* src, size_t rs, int row0, int n, int tid)
+        : at(src + (size_t)(row0 + (tid >> 3)) * rs + (tid & 7) * 8), last(src + (size_t)(n > 0 ? n - 1 : 0) * rs + (tid & 7) * 8), step(64 * rs), row(row0 + (tid >> 3)), n_rows(n) {}
+    __device__ __forceinline__ typename Tr<T>::vec8 next()
+    {
+        const auto x = *reinterpret_cast<const typename Tr<T>::vec8*>(row < n_rows ? at : last);
+        at += step;
+        row += 64;
+        return x;
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void tile_commit(typename Tr<T>::vec8 x, int row0, int n_rows, int tid, T (*dst)[LDS_ROW])
 {
-    if (row0 + 64 > n_rows && row0 + (tid >> 3) >= n_rows) x = typename Tr<T>::vec8{};
+    if (row0 + (tid >> 3) >= n_rows) x = typename Tr<T>::vec8{};
     *reinterpret_cast<typename Tr<T>::vec8*>(&dst[tid >> 3][(tid & 7) * 8]) = x;
 }
 
@@ -52,7 +61,8 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f16v& x0, c
 }
 
 // Both kernels: 8 waves, two a SIMD.  Waves w and w + 4 share a block of 32 rows and take one half each of every 64-row tile of the other side; the second four hand
-// their sums over through LDS at the end, in registers' order.  Tiles are double-buffered: one barrier a tile, loads two tiles ahead.
+// their sums over through LDS at the end, in registers' order.  Tiles are double-buffered: one barrier a tile, loads two tiles ahead, also where those tiles lie
+// behind the end (the last row again): with branches around them, 2304 rows and 10 heads took 51 and 60 us instead of 48 and 57.
 template <typename T> struct Tiles { T a[2][64][LDS_ROW], b[2][64][LDS_ROW]; };
 constexpr int HANDOVER = 4 * 32 * 64 * (int)sizeof(float);   // 4 waves x 32 registers x 64 lanes: fits the tiles' LDS
 static_assert(sizeof(Tiles<__bf16>) >= HANDOVER, "the hand-over uses the tiles' memory");
@@ -117,31 +127,26 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
     float off = 0.f;   // this lane's part of the row's sum of dS
 
     vec8 rk = {}, rv = {};
+    TileRows<T> k_rows(kb, (size_t)g.kv_rs, 0, len, tid), v_rows(vb, (size_t)g.kv_rs, 0, len, tid);
     if (k_hi > 0) {
-        rk = tile_load(kb, (size_t)g.kv_rs, 0, len, tid);
-        rv = tile_load(vb, (size_t)g.kv_rs, 0, len, tid);
+        rk = k_rows.next();
+        rv = v_rows.next();
     }
     fill_bias(g, h, sBias, tid, 512);
     if (k_hi > 0) {
         tile_commit(rk, 0, len, tid, tiles.a[0]);
         tile_commit(rv, 0, len, tid, tiles.b[0]);
-        if (64 < k_hi) {
-            rk = tile_load(kb, (size_t)g.kv_rs, 64, len, tid);
-            rv = tile_load(vb, (size_t)g.kv_rs, 64, len, tid);
-        }
+        rk = k_rows.next();
+        rv = v_rows.next();
     }
     __syncthreads();
     const float far_past = sBias[0] * g.c, far_ahead = sBias[bias_len(g.reach) - 1] * g.c;
     int buf = 0;
     for (int kt = 0; kt < k_hi; kt += 64, buf ^= 1) {
-        if (kt + 64 < k_hi) {
-            tile_commit(rk, kt + 64, len, tid, tiles.a[buf ^ 1]);
-            tile_commit(rv, kt + 64, len, tid, tiles.b[buf ^ 1]);
-            if (kt + 128 < k_hi) {
-                rk = tile_load(kb, (size_t)g.kv_rs, kt + 128, len, tid);
-                rv = tile_load(vb, (size_t)g.kv_rs, kt + 128, len, tid);
-            }
-        }
+        tile_commit(rk, kt + 64, len, tid, tiles.a[buf ^ 1]);
+        tile_commit(rv, kt + 64, len, tid, tiles.b[buf ^ 1]);
+        rk = k_rows.next();
+        rv = v_rows.next();
         const int k0 = kt + half;   // the wave's 32 keys
         f16v s = {}, dp = minus_delta;
         float shift = -L;           // weights are exp2(s c + shift): a single bias of the block goes here
@@ -210,7 +215,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
 {
     typedef typename Tr<T>::vec8 vec8;
     __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: Q, b: dO
-    __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // -lse / c and -delta of a tile's rows: where the accumulators of S and dP start
+    __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // -lse and -delta of a tile's rows
     __shared__ float sFar[8][2];
     __shared__ float sSkew[8][16 * 48];
     extern __shared__ __attribute__((aligned(16))) float sBias[];   // the bias, then 8 arrays of sums by distance
@@ -226,7 +231,6 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     const T* gb = d_o + (size_t)b * g.o_bs + (size_t)h * 64;
     const size_t kvoff = (size_t)b * g.kv_bs + (size_t)h * 64;
     const float* row_b = (wave == 0 ? lse : delta) + (size_t)bh * g.Nq;   // what waves 0 and 1 bring
-    const float row_factor = wave == 0 ? -1.0f / g.c : -1.0f;
 
     const int k0 = tile_y * 128, kw = k0 + (wave & 3) * 32, key = kw + col;
     const bool there = key < len;
@@ -248,48 +252,53 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     const int q_lo = k0 >= len ? g.Nq : (g.causal ? clamp_int(k0 - start, 0, g.Nq) / 64 * 64 : 0);
     vec8 rq = {}, rg = {};
     float rr = 0.f;
-    auto prefetch = [&](int qt) {
-        rq = tile_load(qb, (size_t)g.q_rs, qt, g.Nq, tid);
-        rg = tile_load(gb, (size_t)g.o_rs, qt, g.Nq, tid);
+    TileRows<T> q_rows(qb, (size_t)g.q_rs, q_lo, g.Nq, tid), g_rows(gb, (size_t)g.o_rs, q_lo, g.Nq, tid);
+    auto prefetch = [&](int qt) {   // (tiles in turn)
+        rq = q_rows.next();
+        rg = g_rows.next();
         if (wave < 2) rr = row_b[qt + lane < g.Nq ? qt + lane : g.Nq - 1];
     };
     auto commit = [&](int qt, int buf) {
         tile_commit(rq, qt, g.Nq, tid, tiles.a[buf]);
         tile_commit(rg, qt, g.Nq, tid, tiles.b[buf]);
-        if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? rr * row_factor : (wave == 0 ? -INFINITY : 0.f);   // rows past the end weigh 0
+        if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? -rr : (wave == 0 ? -INFINITY : 0.f);   // rows past the end weigh 0
     };
     if (q_lo < g.Nq) prefetch(q_lo);
     for (int e = tid; e < 8 * blen; e += 512) sBias[blen + e] = 0.f;
     for (int e = lane; e < 16 * 48; e += 64) sSkew[wave][e] = 0.f;
-    fill_bias(g, h, sBias, tid, 512);
+    fill_bias<true>(g, h, sBias, tid, 512);
     if (q_lo < g.Nq) {
         commit(q_lo, 0);
-        if (q_lo + 64 < g.Nq) prefetch(q_lo + 64);
+        prefetch(q_lo + 64);
     }
     __syncthreads();
-    const float far_past = sBias[0] * g.c, far_ahead = sBias[blen - 1] * g.c;
+    const float far_ahead = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sBias[0])));
+    const float far_past = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sBias[blen - 1])));
+    // S starts from the bias; lse is subtracted behind the products, in the exponent: as a start it would be some 1 / c times larger than what is summed, and its
+    // rounding steps with it (a table's gradient in 32 bits at 2304 rows: 1e-6 off, 7e-7 this way, where 32 bits throughout are 7e-7 off).
     int buf = 0;
     for (int qt = q_lo; qt < g.Nq; qt += 64, buf ^= 1) {
-        if (qt + 64 < g.Nq) {
-            commit(qt + 64, buf ^ 1);
-            if (qt + 128 < g.Nq) prefetch(qt + 128);
-        }
+        commit(qt + 64, buf ^ 1);
+        prefetch(qt + 128);
         const int first = start + qt + half;   // position of the block's first query
         const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
         f16v s, dp;
+        f4v minus_lse[4];
 #pragma unroll
         for (int g4 = 0; g4 < 4; g4++) {   // rows 8 g4 + 4 hi + {0 .. 3}
-            const f4v L = *reinterpret_cast<const f4v*>(&sRow[buf][0][half + 8 * g4 + 4 * hi]);
+            minus_lse[g4] = *reinterpret_cast<const f4v*>(&sRow[buf][0][half + 8 * g4 + 4 * hi]);
             const f4v D = *reinterpret_cast<const f4v*>(&sRow[buf][1][half + 8 * g4 + 4 * hi]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) { s[4 * g4 + j] = L[j]; dp[4 * g4 + j] = D[j]; }
+            for (int j = 0; j < 4; j++) dp[4 * g4 + j] = D[j];
         }
-        float shift = 0.f;   // weights are exp2(s c + shift): a single bias of the block goes here
-        const int e0 = key - first - 4 * hi + span - 27;   // row r of the block: e0 + 27 - (r & 3) - 8 (r >> 2)
-        if (past || ahead) shift = past ? far_past : far_ahead;
-        else {
+        if (past || ahead) {
+            const float far = past ? far_past : far_ahead;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] += sBias[e0 + (27 - (r & 3) - 8 * (r >> 2))];
+            for (int r = 0; r < 16; r++) s[r] = far;
+        } else {
+            const float* e = sBias + (first + 4 * hi - key + span);   // (descending distances: row r at + (r & 3) + 8 (r >> 2))
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = e[(r & 3) + 8 * (r >> 2)];
         }
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
@@ -306,7 +315,8 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         unsigned pp[8], pd[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, shift));
+            const f4v L = minus_lse[j >> 1];
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * j], g.c, L[2 * (j & 1)])), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * j + 1], g.c, L[2 * (j & 1) + 1]));
             ds[2 * j] = p0 * dp[2 * j];
             ds[2 * j + 1] = p1 * dp[2 * j + 1];
             pp[j] = Tr<T>::pack2(p0, p1);

@@ -52,14 +52,17 @@ __device__ __forceinline__ float start_value(const Geo& g, float bias)
     return (bias <= -10000.f ? -INFINITY : (bias > 10000.f ? 10000.f : bias)) * g.inv_scale;
 }
 
+// MIRRORED: descending distances, for blocks whose registers run over queries.
+template <bool MIRRORED = false>
 __device__ __forceinline__ void fill_bias(const Geo& g, int h, float* sBias, int tid, int nt)
 {
-    for (int e = tid; e < bias_len(g.reach); e += nt) sBias[e] = start_value(g, table_at(g, bucket_of(g, e - g.reach - PAD), h));
+    for (int e = tid; e < bias_len(g.reach); e += nt) sBias[e] = start_value(g, table_at(g, bucket_of(g, MIRRORED ? g.reach + PAD - e : e - g.reach - PAD), h));
 }
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
-__device__ __forceinline__ int len_of(const Geo& g, int b) { return g.kv_lens ? clamp_int(g.kv_lens[b], 0, g.Nk) : g.Nk; }
-__device__ __forceinline__ int start_of(const Geo& g, int b) { return clamp_int(g.q_starts ? g.q_starts[b] : g.q_start, -(1 << 29), 1 << 29); }
+// (of a batch entry that is the same over a wave: held in scalar registers, so that loops and branches on them are scalar)
+__device__ __forceinline__ int len_of(const Geo& g, int b) { return g.kv_lens ? __builtin_amdgcn_readfirstlane(clamp_int(g.kv_lens[b], 0, g.Nk)) : g.Nk; }
+__device__ __forceinline__ int start_of(const Geo& g, int b) { return __builtin_amdgcn_readfirstlane(clamp_int(g.q_starts ? g.q_starts[b] : g.q_start, -(1 << 29), 1 << 29)); }
 
 // The A operand of a 32x32x16 product from the TRANSPOSE of a row-major LDS tile: lane (m = lane & 31, hi) gets column c0 + m of rows k0 + 8 hi .. + 7.  One
 // transposing read hands each lane of a group of 16 one column of 4 rows x 16 columns, if lane s of the group points at row s / 4, columns 4 (s % 4) .. + 3.
