@@ -199,12 +199,8 @@ __global__ void __launch_bounds__(256) k_adamw32(const Table a, float w1, float 
 
 // x in [0, 448] as e4m3, rounded up with the probability of its distance from the lower neighbour (u: 16 random bits at 4 .. 19).  Scaled by 2^-120 a float's
 // own exponent and upper mantissa bits ARE the code, subnormals of the one becoming subnormals of the other; what is cut off is what the draw is added
-// to, and 448 plus a draw is still 448.  least: the code that a value above 0 has at least.
-__device__ __forceinline__ unsigned to_e4m3(float x, unsigned u, unsigned least)
-{
-    const unsigned b = (__float_as_uint(fminf(x, 448.f) * 0x1p-120f) + u) >> 20;
-    return b < least ? least : b;
-}
+// to, and 448 plus a draw is still 448: also where the product that made x was rounded up, by 15 steps at most.
+__device__ __forceinline__ unsigned to_e4m3(float x, unsigned u) { return (__float_as_uint(x * 0x1p-120f) + u) >> 20; }
 
 // The largest of the wave's values, in all lanes (scalar): over rows of 16, then across the rows, without LDS.
 __device__ __forceinline__ unsigned wave_max(unsigned x)
@@ -289,14 +285,23 @@ __device__ __forceinline__ void chunk8(const gvd_adamw_tensor& t, const Step& st
         const unsigned h0 = (unsigned)i * 0x9D2C5681u + st.key;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const unsigned h = mix(h0 + j * 0x9D2C5681u);
-            unsigned c = to_e4m3(fabsf(mn[j]) * fm, (h << 4) & 0xffff0u, 0u), d = to_e4m3(rn[j] * fr, (h >> 12) & 0xffff0u, rn[j] > 0.f ? 1u : 0u);
-            if (odd) {   // (uniform) what is not finite is held as e4m3's NaN
+            const unsigned h = mix(h0 + j * 0x9D2C5681u), least = min(__float_as_uint(rn[j]), 1u);   // (a root above 0 has code 1 at least)
+            const unsigned c = to_e4m3(fabsf(mn[j]) * fm, (h << 4) & 0xffff0u), d = to_e4m3(rn[j] * fr, (h >> 12) & 0xffff0u);
+            cm |= (c | ((__float_as_uint(mn[j]) >> 24) & 0x80u)) << (8 * j);
+            cr |= max(d, least) << (8 * j);
+        }
+        if (odd) {   // (uniform) what is not finite is held as e4m3's NaN; its code above is arbitrary, in more bits than its own 8: all four anew
+            cm = cr = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned h = mix(h0 + j * 0x9D2C5681u), least = min(__float_as_uint(rn[j]), 1u);
+                unsigned c = to_e4m3(fabsf(mn[j]) * fm, (h << 4) & 0xffff0u), d = to_e4m3(rn[j] * fr, (h >> 12) & 0xffff0u);
+                d = max(d, least);
                 if ((__float_as_uint(mn[j]) & MAGNITUDE) >= NOT_FINITE) c = 0x7fu;
                 if ((__float_as_uint(rn[j]) & MAGNITUDE) >= NOT_FINITE) d = 0x7fu;
+                cm |= (c | ((__float_as_uint(mn[j]) >> 24) & 0x80u)) << (8 * j);
+                cr |= d << (8 * j);
             }
-            cm |= (c | ((__float_as_uint(mn[j]) >> 24) & 0x80u)) << (8 * j);
-            cr |= d << (8 * j);
         }
         store4_bytes<FULL>(m8, i, n, cm);
         store4_bytes<FULL>(r8, i, n, cr);

@@ -9,6 +9,7 @@ import struct
 
 import pytest
 import torch
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 import fused_optim
 from fused_optim import FusedAdamW
@@ -458,6 +459,54 @@ def test_eight_bit_runs_repeat_and_seeds_differ():
         return torch.cat([p.detach().reshape(-1) for p in params]), opt.state[params[0]]["exp_avg"].view(torch.uint8)
     a, b, c = run(1), run(1), run(2)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not torch.equal(a[1], c[1])
+
+
+@gpu
+def test_hooks_schedulers_and_the_profiler_see_each_step():
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    p.grad = torch.full_like(p, 1e-2)
+    seen = []
+    opt = FusedAdamW([p], lr=1e-2)
+    schedule = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.5)
+    opt.step()
+    schedule.step()
+    assert opt.param_groups[0]["lr"] == 5e-3 and not seen
+    before = opt.register_step_pre_hook(lambda o, args, kwargs: seen.append(("before", o is opt, float(o.state[p]["step"]))))
+    after = opt.register_step_post_hook(lambda o, args, kwargs: seen.append(("after", o is opt, float(o.state[p]["step"]))))
+    assert opt.step(lambda: 7.0) == 7.0
+    assert seen == [("before", True, 1.0), ("after", True, 2.0)]
+    before.remove()
+    after.remove()
+    opt.step()
+    assert len(seen) == 2 and float(opt.state[p]["step"]) == 3
+    every = register_optimizer_step_post_hook(lambda o, args, kwargs: seen.append("every"))
+    opt.step()
+    every.remove()
+    assert seen[2:] == ["every"]
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any(e.key == "Optimizer.step#FusedAdamW.step" for e in prof.key_averages())
+    assert float(opt.state[p]["step"]) == 5
+
+
+@gpu
+def test_nothing_is_counted_where_a_later_launch_is_refused():
+    a, b = (torch.nn.Parameter(torch.ones(64, device=DEV, dtype=t)) for t in (torch.float32, torch.bfloat16))
+    opt = FusedAdamW([a, b], lr=1e-2)
+    for p in (a, b):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept = a.detach().clone()
+    opt.state[b]["exp_avg"] = torch.zeros(63, device=DEV)
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        opt.step()
+    assert float(opt.state[a]["step"]) == 1 and torch.equal(a, kept)
+    opt.state[b]["exp_avg"] = "none"
+    with pytest.raises(RuntimeError, match="no tensor"):
+        opt.step()
+    opt.state[b] = {}                   # set up anew
+    opt.step()
+    assert float(opt.state[a]["step"]) == 2 and float(opt.state[b]["step"]) == 1 and not torch.equal(a, kept)
 
 
 # ---- capture and streams ----------------------------------------------------------------------------------------------------------
