@@ -1,11 +1,15 @@
-// relattn_torch_ext.cpp -- relative_bias_attention as one torch::autograd::Function over the C-ABI (include/gvd_relattn.h): checks of arguments, strides, outputs,
+// relattn_torch_ext.cpp -- relative_bias_attention as one node of the autograd graph over the C-ABI (include/gvd_relattn.h): checks of arguments, strides, outputs,
 // workspaces, and the backward without Python.  No kernel lives here.  With a Python autograd function a training pass took 180 us of host time, as much
-// as its kernels at the sizes of a temporal layer.
+// as its kernels at the sizes of a temporal layer; with torch::autograd::Function 80, as a node of its own PASS_US (30 of them the engine's, for any graph).
 //
 // Plain C++ (g++); the entry points are resolved from the library path that Python hands to init(), so A/B builds share one instance.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
@@ -117,46 +121,80 @@ at::Tensor forward_(at::Tensor q, at::Tensor k, at::Tensor v, const at::Tensor& 
     return out;
 }
 
-struct RelativeBiasAttention : torch::autograd::Function<RelativeBiasAttention> {
-    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& table,
-                              const Config& c)
-    {
-        const at::Tensor q = packed(q_), k = packed(k_), v = packed(v_);
-        at::Tensor lse;
-        const at::Tensor out = forward_(q, k, v, table, at::Tensor(), c, &lse);
-        torch::autograd::variable_list saved = {q, k, v, table, out, lse};
-        if (c.kv_lens.defined()) saved.push_back(c.kv_lens);
-        ctx->save_for_backward(saved);
-        ctx->saved_data["first"] = c.first;
-        ctx->saved_data["heads"] = c.heads;
-        ctx->saved_data["q_start"] = c.q_start;
-        ctx->saved_data["flags"] = (int64_t)(c.both | c.causal << 1 | c.frame_major << 2);
-        ctx->saved_data["scale"] = c.scale;
-        return out;
-    }
+struct RelativeBiasAttentionBackward : torch::autograd::Node {
+    torch::autograd::SavedVariable q, k, v, table, out, kv_lens;
+    at::Tensor lse;
+    Config c;   // (kv_lens aside)
 
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads)
+    std::string name() const override { return "RelativeBiasAttentionBackward"; }
+    void release_variables() override
+    {
+        for (torch::autograd::SavedVariable* x : {&q, &k, &v, &table, &out, &kv_lens}) x->reset_data();
+        lse.reset();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override
     {
         TORCH_CHECK(!at::GradMode::is_enabled(), "relative_bias_attention: its gradients have no gradients (create_graph=True)");
-        const auto saved = ctx->get_saved_variables();
-        const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &out = saved[4], &lse = saved[5];
-        const int64_t flags = ctx->saved_data["flags"].toInt();
-        const Config c = {ctx->saved_data["first"].toTensor(), saved.size() > 6 ? saved[6] : at::Tensor(), ctx->saved_data["heads"].toInt(), ctx->saved_data["q_start"].toInt(), (flags & 1) != 0, (flags & 2) != 0,
-                          (flags & 4) != 0, ctx->saved_data["scale"].toDouble()};
-        const c10::DeviceGuard guard(q.device());
-        at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dtable = at::empty_like(table);
-        if (q.numel() == 0 || k.numel() == 0) {
+        if (!grads[0].defined()) return torch::autograd::variable_list(4);
+        Config c_ = c;
+        const at::Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), table_ = table.unpack(), out_ = out.unpack(shared_from_this());
+        c_.kv_lens = kv_lens.unpack();
+        const c10::DeviceGuard guard(q_.device());
+        at::AutoDispatchBelowAutograd below;
+        at::Tensor dq = at::empty_like(q_), dk = at::empty_like(k_), dv = at::empty_like(v_), dtable = at::empty_like(table_);
+        if (q_.numel() == 0 || k_.numel() == 0) {
             for (at::Tensor* t : {&dq, &dk, &dv, &dtable}) t->zero_();
         } else {
             const at::Tensor g = packed(grads[0]);
-            const gvd_relattn_problem p = problem(q, k, out, table, at::Tensor(), c);
-            const at::Tensor ws = bytes(check(g_api.bwd_workspace(&p)), q);
-            check(g_api.bwd(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
-                            dv.data_ptr(), dtable.data_ptr(), ptr(ws), stream_of(q)));
+            const gvd_relattn_problem p = problem(q_, k_, out_, table_, at::Tensor(), c_);
+            const at::Tensor ws = bytes(check(g_api.bwd_workspace(&p)), q_);
+            check(g_api.bwd(&p, q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), table_.data_ptr(), out_.data_ptr(), g.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
+                            dv.data_ptr(), dtable.data_ptr(), ptr(ws), stream_of(q_)));
         }
-        return {dq, dk, dv, dtable, at::Tensor()};
+        return {dq, dk, dv, dtable};
     }
 };
+
+// A leaf's accumulating node belongs to the stream that it was made on and lives as long as some graph of the leaf does.  A backward pass that is captured while an
+// eager graph of the same leaf lives would make that stream wait for a captured one, in the engine's thread, where the error ends the process: refused here, before.
+void refuse_foreign_accumulators(std::initializer_list<const at::Tensor*> inputs, const at::Device& device)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()).stream(), &capture) == hipSuccess, "relative_bias_attention: the stream cannot be asked whether it is capturing");
+    if (capture == hipStreamCaptureStatusNone) return;
+    const c10::Stream now = c10::impl::VirtualGuardImpl(device.type()).getStream(device);
+    for (const at::Tensor* t : inputs) {
+        if (!t->requires_grad() || !t->is_leaf()) continue;
+        const auto accumulate = torch::autograd::impl::try_get_grad_accumulator(*t);
+        TORCH_CHECK(!accumulate || !accumulate->stream() || *accumulate->stream() == now,
+                    "relative_bias_attention: a training pass cannot be captured while an eager graph of the same leaf lives (drop its outputs first, or run it on the "
+                    "capturing stream)");
+    }
+}
+
+at::Tensor differentiable(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& table, const Config& c)
+{
+    for (const at::Tensor* t : {&q_, &k_, &v_, &table})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "relative_bias_attention: no forward-mode derivatives");
+    const std::shared_ptr<RelativeBiasAttentionBackward> node(new RelativeBiasAttentionBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q_, k_, v_, table));
+    at::Tensor out;
+    {
+        at::AutoDispatchBelowAutograd below;
+        const at::Tensor q = packed(q_), k = packed(k_), v = packed(v_);
+        out = forward_(q, k, v, table, at::Tensor(), c, &node->lse);
+        node->q = torch::autograd::SavedVariable(q, false);
+        node->k = torch::autograd::SavedVariable(k, false);
+        node->v = torch::autograd::SavedVariable(v, false);
+    }
+    node->table = torch::autograd::SavedVariable(table, false);
+    node->kv_lens = torch::autograd::SavedVariable(c.kv_lens, false);
+    node->c = c;
+    node->c.kv_lens.reset();
+    torch::autograd::set_history(out, node);
+    node->out = torch::autograd::SavedVariable(out, true);
+    return out;
+}
 
 #define GVD_WANT(cond, ...) TORCH_CHECK_VALUE(cond, "relative_bias_attention: ", __VA_ARGS__)
 
@@ -188,7 +226,8 @@ at::Tensor attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Ten
             k = k.expand(shape);
             v = v.expand(shape);
         }
-        return RelativeBiasAttention::apply(q, k, v, table, c);
+        refuse_foreign_accumulators({&q, &k, &v, &table}, q.device());
+        return differentiable(q, k, v, table, c);
     }
     return forward_(q, k, v, table, q_starts, c, nullptr);
 }

@@ -504,6 +504,39 @@ def test_replays_equal_eager_calls(shape):
 
 
 @gpu
+@pytest.mark.parametrize("n", [25, 300])
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(n):
+    """Refused in the forward, before there is a backward to capture; the capture goes on without it, and works once the eager graph is gone."""
+    H = 3
+    q, k, v = (torch.randn(2, n, H * D, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    table = torch.randn(32, H, device=DEV, requires_grad=True)
+    g = torch.randn_like(q)
+    eager = ops.relative_bias_attention(q, k, v, table, H)          # lives on
+    want, = torch.autograd.grad(eager, [table], g, retain_graph=True)
+    side = torch.cuda.Stream()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph, stream=side):
+        x += 1
+        with pytest.raises(RuntimeError, match="eager graph"):
+            ops.relative_bias_attention(q, k, v, table, H)
+        with torch.no_grad():
+            y = ops.relative_bias_attention(q, k, v, table, H)      # inference is no concern
+    graph.replay()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        assert torch.equal(y, ops.relative_bias_attention(q, k, v, table, H)) and float(x[0]) == 1
+    del eager
+    graph2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2, stream=side):
+        got, = torch.autograd.grad(ops.relative_bias_attention(q, k, v, table, H), [table], g)
+    for _ in range(3):
+        got.zero_()
+        graph2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@gpu
 @pytest.mark.parametrize("n", [25, 200])
 def test_a_captured_training_pass_replays(n):
     q, k, v, t, g = inputs(2, 2, n, n, torch.bfloat16)
