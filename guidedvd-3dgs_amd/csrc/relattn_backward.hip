@@ -407,7 +407,16 @@ __global__ void __launch_bounds__(64) k_rel_table(const float* __restrict__ part
 {
     const int bucket = blockIdx.x, h = blockIdx.y;
     double x = 0.0;
-    for (int j = threadIdx.x; j < count; j += 64) x += (double)part[(((size_t)(j / tiles) * H + h) * tiles + j % tiles) * buckets + bucket];
+    for (int j0 = threadIdx.x; j0 < count; j0 += 512) {   // eight loads in flight
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int j = j0 + 64 * i;
+            y[i] = j < count ? part[(((size_t)(j / tiles) * H + h) * tiles + j % tiles) * buckets + bucket] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) x += (double)y[i];
+    }
 #pragma unroll
     for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w, 64);
     if (threadIdx.x == 0) dtable[bucket * H + h] = (E)(float)x;
