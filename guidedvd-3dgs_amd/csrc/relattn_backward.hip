@@ -19,12 +19,13 @@ using namespace gvdr;
 
 namespace {
 
-// Tiles of 64 rows x 64 channels in turn, through 512 lanes, 16 bytes each: eight lanes a row.  Rows at or behind n_rows: the last one again (n_rows >= 1), and zeros
-// in LDS.  The address moves along: a row's number times the stride, in 64 bits, would take the vector unit as long as 40 additions a lane and tile.
+// Tiles of 64 rows x 64 channels in turn, through 512 lanes, 16 bytes each: eight lanes a row.  Rows at or behind n_rows: the last one again (n_rows >= 1).
+// The address moves along: a row's number times the stride, in 64 bits, would take the vector unit as long as 40 additions a lane and tile.
 template <typename T> struct TileRows {
     const T *at, *last;
     size_t step;
     int row, n_rows;
+
     __device__ __forceinline__ TileRows(const T* src, size_t rs, int row0, int n, int tid)
         : at(src + (size_t)(row0 + (tid >> 3)) * rs + (tid & 7) * 8), last(src + (size_t)(n > 0 ? n - 1 : 0) * rs + (tid & 7) * 8), step(64 * rs), row(row0 + (tid >> 3)), n_rows(n) {}
     __device__ __forceinline__ typename Tr<T>::vec8 next()
@@ -37,9 +38,8 @@ template <typename T> struct TileRows {
 };
 
 template <typename T>
-__device__ __forceinline__ void tile_commit(typename Tr<T>::vec8 x, int row0, int n_rows, int tid, T (*dst)[LDS_ROW])
+__device__ __forceinline__ void tile_commit(typename Tr<T>::vec8 x, int tid, T (*dst)[LDS_ROW])
 {
-    if (row0 + (tid >> 3) >= n_rows) x = typename Tr<T>::vec8{};
     *reinterpret_cast<typename Tr<T>::vec8*>(&dst[tid >> 3][(tid & 7) * 8]) = x;
 }
 
@@ -62,7 +62,9 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f16v& x0, c
 
 // Both kernels: 8 waves, two a SIMD.  Waves w and w + 4 share a block of 32 rows and take one half each of every 64-row tile of the other side; the second four hand
 // their sums over through LDS at the end, in registers' order.  Tiles are double-buffered: one barrier a tile, loads two tiles ahead, also where those tiles lie
-// behind the end (the last row again): with branches around them, 2304 rows and 10 heads took 51 and 60 us instead of 48 and 57.
+// behind the end: with branches around them, 2304 rows and 10 heads took 51 and 60 us instead of 48 and 57.  Rows at or behind the end come as the last one again and
+// weigh 0 (the bias of -infinity they meet is set in registers; zeros in LDS instead: 3 us more).  Where in the loop the next tile's stores to LDS stand was measured,
+// place by place: before the second products in k_rel_dq (43.8 us; first thing 45.3, last 49.7), last in k_rel_dkv (54.5; 55.6, 56.4 before the sums).
 template <typename T> struct Tiles { T a[2][64][LDS_ROW], b[2][64][LDS_ROW]; };
 constexpr int HANDOVER = 4 * 32 * 64 * (int)sizeof(float);   // 4 waves x 32 registers x 64 lanes: fits the tiles' LDS
 static_assert(sizeof(Tiles<__bf16>) >= HANDOVER, "the hand-over uses the tiles' memory");
@@ -134,8 +136,8 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
     }
     fill_bias(g, h, sBias, tid, 512);
     if (k_hi > 0) {
-        tile_commit(rk, 0, len, tid, tiles.a[0]);
-        tile_commit(rv, 0, len, tid, tiles.b[0]);
+        tile_commit(rk, tid, tiles.a[0]);
+        tile_commit(rv, tid, tiles.b[0]);
         rk = k_rows.next();
         rv = v_rows.next();
     }
@@ -143,10 +145,6 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
     const float far_past = sBias[0] * g.c, far_ahead = sBias[bias_len(g.reach) - 1] * g.c;
     int buf = 0;
     for (int kt = 0; kt < k_hi; kt += 64, buf ^= 1) {
-        tile_commit(rk, kt + 64, len, tid, tiles.a[buf ^ 1]);
-        tile_commit(rv, kt + 64, len, tid, tiles.b[buf ^ 1]);
-        rk = k_rows.next();
-        rv = v_rows.next();
         const int k0 = kt + half;   // the wave's 32 keys
         f16v s = {}, dp = minus_delta;
         float shift = -L;           // weights are exp2(s c + shift): a single bias of the block goes here
@@ -158,16 +156,15 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
             for (int r = 0; r < 16; r++) s[r] = e[(r & 3) + 8 * (r >> 2)];
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), qf[ks], s);
-            dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), gf[ks], dp);
-        }
+        for (int ks = 0; ks < 4; ks++) s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), qf[ks], s);
         if (k0 + 32 > k_full) {
             const int seen = (g.causal && start + query + 1 < len ? start + query + 1 : len) - k0 - 4 * hi;
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 if ((r & 3) + 8 * (r >> 2) >= seen) s[r] = -INFINITY;
         }
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), gf[ks], dp);
         unsigned pp[8], pd[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -177,9 +174,13 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
             pp[j] = Tr<T>::pack2(p0, p1);
             pd[j] = Tr<T>::pack2(d0, d1);
         }
+        tile_commit(rk, tid, tiles.a[buf ^ 1]);
+        tile_commit(rv, tid, tiles.b[buf ^ 1]);
+        rk = k_rows.next();
+        rv = v_rows.next();
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 df = packed_c_to_b_operand<T>(pd, k2), pf = packed_c_to_b_operand<T>(pp, k2);
+            const vec8 df = packed_operand<T>(pd, k2), pf = packed_operand<T>(pp, k2);
             const vec8 a0 = transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane);
             const vec8 a1 = transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane);
             dq0 = Tr<T>::mfma(a0, df, dq0);
@@ -259,8 +260,8 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         if (wave < 2) rr = row_b[qt + lane < g.Nq ? qt + lane : g.Nq - 1];
     };
     auto commit = [&](int qt, int buf) {
-        tile_commit(rq, qt, g.Nq, tid, tiles.a[buf]);
-        tile_commit(rg, qt, g.Nq, tid, tiles.b[buf]);
+        tile_commit(rq, tid, tiles.a[buf]);
+        tile_commit(rg, tid, tiles.b[buf]);
         if (wave < 2) sRow[buf][wave][lane] = qt + lane < g.Nq ? -rr : (wave == 0 ? -INFINITY : 0.f);   // rows past the end weigh 0
     };
     if (q_lo < g.Nq) prefetch(q_lo);
@@ -278,8 +279,6 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     // rounding steps with it (a table's gradient in 32 bits at 2304 rows: 1e-6 off, 7e-7 this way, where 32 bits throughout are 7e-7 off).
     int buf = 0;
     for (int qt = q_lo; qt < g.Nq; qt += 64, buf ^= 1) {
-        commit(qt + 64, buf ^ 1);
-        prefetch(qt + 128);
         const int first = start + qt + half;   // position of the block's first query
         const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
         f16v s, dp;
@@ -301,16 +300,15 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
             for (int r = 0; r < 16; r++) s[r] = e[(r & 3) + 8 * (r >> 2)];
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), kf[ks], s);
-            dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), vf[ks], dp);
-        }
+        for (int ks = 0; ks < 4; ks++) s = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.a[buf][half + col][16 * ks + 8 * hi]), kf[ks], s);
         if (kw + 32 > len || (g.causal && kw + 31 > first)) {
             const int least = !there ? 0x7fffffff : (g.causal ? key - first - 4 * hi : -64);   // the key's first row that sees it
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 if ((r & 3) + 8 * (r >> 2) < least) s[r] = -INFINITY;
         }
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) dp = Tr<T>::mfma(*reinterpret_cast<const vec8*>(&tiles.b[buf][half + col][16 * ks + 8 * hi]), vf[ks], dp);
         float ds[16];
         unsigned pp[8], pd[8];
 #pragma unroll
@@ -344,12 +342,14 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         }
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 pf = packed_c_to_b_operand<T>(pp, k2), df = packed_c_to_b_operand<T>(pd, k2);
+            const vec8 pf = packed_operand<T>(pp, k2), df = packed_operand<T>(pd, k2);
             dv0 = Tr<T>::mfma(transposed_operand(&tiles.b[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), pf, dv0);
             dv1 = Tr<T>::mfma(transposed_operand(&tiles.b[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), pf, dv1);
             dk0 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 0, lane), df, dk0);
             dk1 = Tr<T>::mfma(transposed_operand(&tiles.a[buf][0][0], LDS_ROW, half + 16 * k2, 32, lane), df, dk1);
         }
+        commit(qt + 64, buf ^ 1);
+        prefetch(qt + 128);
         __syncthreads();
     }
     float* at = reinterpret_cast<float*>(&tiles);
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
         f16v a0 = {}, a1 = {};
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 df = packed_c_to_b_operand<T>(pdT, k2);
+            const vec8 df = packed_operand<T>(pdT, k2);
             a0 = Tr<T>::mfma(transposed_operand(&sK[wave][0][0], OP, 16 * k2, 0, lane), df, a0);
             a1 = Tr<T>::mfma(transposed_operand(&sK[wave][0][0], OP, 16 * k2, 32, lane), df, a1);
         }
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
         f16v dv0 = {}, dv1 = {}, dk0 = {}, dk1 = {};
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 pf = packed_c_to_b_operand<T>(pp, k2), df = packed_c_to_b_operand<T>(pd, k2);
+            const vec8 pf = packed_operand<T>(pp, k2), df = packed_operand<T>(pd, k2);
             dv0 = Tr<T>::mfma(transposed_operand(&sG[wave][0][0], OP, 16 * k2, 0, lane), pf, dv0);
             dv1 = Tr<T>::mfma(transposed_operand(&sG[wave][0][0], OP, 16 * k2, 32, lane), pf, dv1);
             dk0 = Tr<T>::mfma(transposed_operand(&sQ[wave][0][0], OP, 16 * k2, 0, lane), df, dk0);

@@ -64,16 +64,28 @@ __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo 
 __device__ __forceinline__ int len_of(const Geo& g, int b) { return g.kv_lens ? __builtin_amdgcn_readfirstlane(clamp_int(g.kv_lens[b], 0, g.Nk)) : g.Nk; }
 __device__ __forceinline__ int start_of(const Geo& g, int b) { return __builtin_amdgcn_readfirstlane(clamp_int(g.q_starts ? g.q_starts[b] : g.q_start, -(1 << 29), 1 << 29)); }
 
-// The A operand of a 32x32x16 product from the TRANSPOSE of a row-major LDS tile: lane (m = lane & 31, hi) gets column c0 + m of rows k0 + 8 hi .. + 7.  One
+// A product's result as the next product's operand.  Of a 32 x 32 block a lane of half hi holds rows 4 hi + {0 .. 3, 8 .. 11, 16 .. 19, 24 .. 27} of one column, in registers'
+// order; the matrix unit wants eight of the contraction's indexes a lane and step of 16, WHICH ones is free as long as both operands agree.  So the block goes on as it
+// lies, registers 8 k2 .. + 7 packed, and the other operand brings rows 4 hi + {0 .. 3, 8 .. 11} of each 16: nothing is exchanged between the halves (that
+// took 8 instructions a block).
+template <typename T>
+__device__ __forceinline__ typename Tr<T>::vec8 packed_operand(const unsigned (&pk)[8], int k2)
+{
+    typedef unsigned u4_ __attribute__((ext_vector_type(4)));
+    const u4_ x = { pk[4 * k2], pk[4 * k2 + 1], pk[4 * k2 + 2], pk[4 * k2 + 3] };
+    return __builtin_bit_cast(typename Tr<T>::vec8, x);
+}
+
+// ... and that other operand from the TRANSPOSE of a row-major LDS tile: lane (m = lane & 31, hi) gets column c0 + m of rows k0 + 4 hi + {0 .. 3, 8 .. 11}.  One
 // transposing read hands each lane of a group of 16 one column of 4 rows x 16 columns, if lane s of the group points at row s / 4, columns 4 (s % 4) .. + 3.
 // (Writing tiles a second time, transposed, took 6 dword writes and 2 more loads a lane and tile.)
 template <typename T>
 __device__ __forceinline__ typename Tr<T>::vec8 transposed_operand(const T* tile, int pitch, int k0, int c0, int lane)
 {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    const T* p = tile + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * pitch + c0 + (lane & 16) + 4 * (lane & 3);
+    const T* p = tile + (k0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * pitch + c0 + (lane & 16) + 4 * (lane & 3);
     const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 4 * pitch));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(p + 8 * pitch));
     return __builtin_bit_cast(typename Tr<T>::vec8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 

@@ -251,7 +251,7 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
                 const vec8 v1 = transposed_operand(&sVb[buf][0][0], LDS_ROW, 32 * kbk + 16 * k2, 32, lane);
 #pragma unroll
                 for (int qi = 0; qi < QB; qi++) {
-                    const vec8 pf = packed_c_to_b_operand<T>(kbk == 0 ? pk0[qi] : pk1[qi], k2);
+                    const vec8 pf = packed_operand<T>(kbk == 0 ? pk0[qi] : pk1[qi], k2);
                     o0[qi] = Tr<T>::mfma(v0, pf, o0[qi]);
                     o1[qi] = Tr<T>::mfma(v1, pf, o1[qi]);
                 }
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
         f16v o0 = {}, o1 = {};
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const vec8 pf = packed_c_to_b_operand<T>(pk, k2);
+            const vec8 pf = packed_operand<T>(pk, k2);
             o0 = Tr<T>::mfma(transposed_operand(&rows[0][0], PITCH, 16 * k2, 0, lane), pf, o0);
             o1 = Tr<T>::mfma(transposed_operand(&rows[0][0], PITCH, 16 * k2, 32, lane), pf, o1);
         }
