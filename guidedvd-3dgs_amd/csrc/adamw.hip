@@ -5,7 +5,7 @@
 // Bound by memory: every element is read and written once -- 28 bytes with 32-bit moments and fp32 parameters, 16 with 8-bit ones -- and no
 // element depends on another (with 8-bit moments: on its block of 256).  So: one launch for up to MAX_TENSORS tensors (their table travels in
 // the kernel's arguments: nothing to upload, nothing that a captured graph could find changed), workgroups of CHUNK consecutive elements,
-// 16-byte accesses.  118M fp32 elements: 562 us, 5.9 TB/s (a plain copy of that size reaches 4.9); 11.8M with 8-bit moments: 34 us, 5.6 TB/s.
+// 16-byte accesses.  118M fp32 elements: 560 us, 5.9 TB/s (a plain copy of that size reaches 4.9); 11.8M with 8-bit moments: 33 us, 5.7 TB/s.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 (4 significant bits, 2^-9 .. 448) with one scale a block of 256 consecutive elements
 // (largest magnitude / 448), a block per wave.  Two choices carry this:

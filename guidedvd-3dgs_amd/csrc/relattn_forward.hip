@@ -75,7 +75,8 @@ int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who)
 namespace {
 
 // ---- general rows ------------------------------------------------------------------------------------------------------------
-// The vector unit bounds this kernel: 32 exponentials a lane, query block and tile (quarter rate), against 16 products of the matrix unit.  So the loop does little else:
+// The vector unit bounds this kernel: 32 exponentials a lane, query block and tile, against 16 products of the matrix unit.  9216 rows, 5 heads: 147 us, 740 TFLOP/s; 20 heads
+// 540, 805; 2304 rows, 10 heads: 37.  So the loop does little else:
 //   * the maximum is not looked for: weights are formed with the running one, and a row sum above 2^15 (always for the first tile: the maximum starts
 //     below every score) sends the block through the exact path.  Numerators and denominator share the maximum, so any one that keeps weights finite
 //     gives the exact softmax;
@@ -481,8 +482,8 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
 
 // ---- few queries, many keys ----------------------------------------------------------------------------------------------------
 // 8 lanes hold a key's 64 channels, a wave 8 keys at once, 4 of those in flight; every lane group keeps its own running maximum and sum, joined at the end.
-// 16 x 10 rows against caches of 8192 (half full on average): 41 us with the join, 4.3 TB/s; with ordinary loads 45, with an item's parts on one XCD 3 more, with
-// 8 workgroups a CU 41 (and 64 x 20 rows against 1000: 39 against 36), with 8 keys a lane group in flight 63.
+// 16 x 10 rows against caches of 8192 (half full on average): 37 us with the join, 4.8 TB/s.  (When these were tried it was 41: with ordinary loads 45, with an item's
+// parts on one XCD 3 more, with 8 workgroups a CU 41 -- and 64 x 20 rows against 1000: 39 against 36 --, with 8 keys a lane group in flight 63.)
 template <typename T, int NQ>
 __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
                                                  float* __restrict__ lse, float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
@@ -613,8 +614,9 @@ struct Plan { Form form; int qb, tiles, parts; };
 // Which kernel, how many query blocks a wave, and into how many parts the keys are cut.
 // General rows: what a choice takes is estimated, in microseconds, and the least is taken.  A workgroup of 128 rows takes 0.95 a tile alone on its CU and 0.745 with
 // others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products); a round of workgroups starts with 4 (bias, first tiles); parts
-// take 8 (their stores, the join's launch) and 3.3e-5 a row and part.  Measured against it (us): 9216 queries and keys, 5 heads: 128 rows 214, in 2 parts 170; 256 rows 219, in 2 parts
-// 190, in 4 parts 162.  2304, 10 heads: 128 rows 39, 256 rows 58, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 48.5, in 2 parts 55; 256 rows 51.
+// take 8 (their stores, the join's launch) and 3.3e-5 a row and part.  Measured, with the join (us): 9216 queries and keys, 5 heads: 128 rows 212, in 2 parts 162; 256 rows 212, in 2 parts
+// 186, in 4 parts 157.  2304, 10 heads: 128 rows 37, 256 rows 55, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 41, in 2 parts 53; 256 rows 48.  Over ten
+// shapes and eight choices each, what it picks is 0.5 % off the best on average, 3 % at most.
 Plan plan_of(const Geo& g, int B, int cus)
 {
     const long long bh = (long long)B * g.H;

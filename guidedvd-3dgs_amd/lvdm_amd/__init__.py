@@ -7,6 +7,7 @@
     conv       the hand-written MFMA convolutions (3x3, upsample, temporal) behind unet / vae
     guidance   B12  LossGuidance
     model      B1/B5 LatentDiffusion-shaped wrapper the samplers duck-type against (apply_model, decode)
+    relative   attention with a learned relative position bias (ops.relative_bias_attention)
     ops        hot operators; HIP kernels (csrc/*.hip) on ROCm devices, no silent CPU fallback
 
 Importing this package changes no process-wide state, and nothing in it configures a vendor library: since round 4 no hipBLASLt /
