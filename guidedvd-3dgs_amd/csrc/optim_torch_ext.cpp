@@ -153,6 +153,9 @@ struct Launch {
         check(g_api.step(table.data(), (int)n, param_type(), (int)bits, beta1, beta2, eps, capturable ? scalars.data_ptr() : nullptr, stream()));
         if (!capturable)
             for (size_t i = 0; i < n; i++) ++*flat[i * k + 2].data_ptr<float>();   // (counted once the launch stands)
+        // all were written behind autograd's back: graphs that saved them, and images that were packed from them, go by their version
+        for (size_t i = 0; i < flat.size(); i++)
+            if (i % k != 1 && !flat[i].is_inference()) flat[i].unsafeGetTensorImpl()->bump_version();
     }
 };
 

@@ -171,8 +171,7 @@ void refuse_foreign_accumulators(std::initializer_list<const at::Tensor*> inputs
         if (!t->requires_grad() || !t->is_leaf()) continue;
         const auto accumulate = torch::autograd::impl::try_get_grad_accumulator(*t);
         TORCH_CHECK(!accumulate || !accumulate->stream() || *accumulate->stream() == now,
-                    "relative_bias_attention: a training pass cannot be captured while an eager graph of the same leaf lives (drop its outputs first, or run it on the "
-                    "capturing stream)");
+                    "relative_bias_attention: a training pass cannot be captured while an eager graph of the same leaf lives (drop its outputs first)");
     }
 }
 

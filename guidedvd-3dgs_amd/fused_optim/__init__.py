@@ -84,7 +84,8 @@ class FusedAdamW(torch.optim.Optimizer):
                  "exp_avg", "exp_avg_rms" (float8_e4m3fn), "exp_avg_scale", "exp_avg_rms_scale".
     capturable   the count of steps is held on the device ("step": float32 there), and step() may be captured into a graph, where every replay is
                  the next step; lr may be a float32 tensor of one element on the parameters' device, read at each replay.  Run one eager step
-                 first: state cannot be set up while capturing.  Without it step() raises in a capture: the count would be frozen."""
+                 first: state cannot be set up while capturing.  Without it step() raises in a capture: the count would be frozen.  A replay leaves the
+                 parameters' version counters as they are: after replays, `lvdm_amd.conv.invalidate_packed` for modules whose images are cached."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0, capturable=False):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed,

@@ -509,6 +509,39 @@ def test_nothing_is_counted_where_a_later_launch_is_refused():
     assert float(opt.state[a]["step"]) == 2 and float(opt.state[b]["step"]) == 1 and not torch.equal(a, kept)
 
 
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_versions_count_each_step(bits):
+    """Graphs that saved a parameter refuse it afterwards, and images packed from it are packed anew."""
+    from lvdm_amd import gemm
+    lin = torch.nn.Linear(320, 320).half().to(DEV)
+    x = torch.randn(512, 320, device=DEV).half()
+    opt = FusedAdamW(lin.parameters(), lr=0.1, weight_decay=0.0, state_bits=bits)
+
+    def check():
+        with torch.no_grad():
+            y = gemm.linear(x, lin.weight, lin.bias).double()
+        X, W, b = x.double(), lin.weight.detach().double(), lin.bias.detach().double()
+        want = X @ W.t() + b
+        assert bool(((y - want).abs() <= 2.0 ** -11 * want.abs() + 321 * U * (X.abs() @ W.abs().t() + b.abs())).all())   # rounded once; sums in 32 bits
+        return y
+    first = check()
+    saved = (lin.weight.float() * lin.weight.float()).sum()
+    held = (lin.weight * lin.weight).sum()
+    before = [p._version for p in lin.parameters()]
+    for p in lin.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert all(p._version > v for p, v in zip(lin.parameters(), before))
+    assert float((check() - first).abs().max()) > 1
+    saved.backward()                                    # (its graph saved copies)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        held.backward()
+    state = {k: v._version for k, v in opt.state[lin.weight].items()}
+    opt.step()
+    assert all(opt.state[lin.weight][k]._version > v for k, v in state.items())
+
+
 # ---- capture and streams ----------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])

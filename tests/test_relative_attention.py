@@ -537,6 +537,63 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(n):
 
 
 @gpu
+def test_a_captured_pass_of_two_layers_that_share_a_table_replays():
+    """The second use of the table meets its accumulating node, made in the same capture."""
+    H, n = 3, 70
+    q, k, v = (torch.randn(2, n, H * D, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    table = torch.randn(32, H, device=DEV, requires_grad=True)
+
+    def one():
+        x = ops.relative_bias_attention(q, k, v, table, H)
+        y = ops.relative_bias_attention(x, k, v, table, H, causal=True)
+        got, = torch.autograd.grad(y, [table], torch.ones_like(y))
+        return y.detach(), got
+    one()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, got = one()
+    for rep in range(4):
+        q.copy_(torch.randn(q.shape, device=DEV))
+        graph.replay()
+        want = one()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(got, want[1]), rep
+
+
+@gpu
+@pytest.mark.parametrize("n", [25, 70])
+def test_the_graph_is_an_ordinary_one(n):
+    """A second pass over a kept graph, none over a freed one, none over inputs changed in place; gradients of some inputs only; no second derivatives."""
+    H = 2
+    q, k, v, t, g = inputs(2, H, n, n, torch.bfloat16)
+    lens = torch.tensor([n, n // 2], dtype=torch.int32, device=DEV)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, t)]
+    out = ops.relative_bias_attention(*leaves, H, kv_lens=lens)
+    first = torch.autograd.grad(out, leaves, g, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, g)
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+    with pytest.raises(RuntimeError, match="second time|freed"):
+        torch.autograd.grad(out, leaves, g)
+    for i in range(4):
+        some = [x.detach().requires_grad_(j == i) for j, x in enumerate((q, k, v, t))]
+        got, = torch.autograd.grad(ops.relative_bias_attention(*some, H, kv_lens=lens), [some[i]], g)
+        assert torch.equal(got, first[i])
+    for changed in (leaves[1], lens):
+        out = ops.relative_bias_attention(*leaves, H, kv_lens=lens)
+        with torch.no_grad():
+            changed.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaves, g)
+    out = ops.relative_bias_attention(*leaves, H)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out, leaves, g, create_graph=True)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(leaves[0], torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.relative_bias_attention(dual, *leaves[1:], H)
+
+
+@gpu
 @pytest.mark.parametrize("n", [25, 200])
 def test_a_captured_training_pass_replays(n):
     q, k, v, t, g = inputs(2, 2, n, n, torch.bfloat16)
