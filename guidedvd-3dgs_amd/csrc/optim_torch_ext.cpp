@@ -227,7 +227,7 @@ void step(const py::object& optimizer, const py::list& groups, const py::dict& s
             const at::Tensor& p = THPVariable_Unpack(p_);
             const at::Tensor& grad = p.grad();
             if (!grad.defined()) continue;
-            TORCH_CHECK(p.is_cuda(), "FusedAdamW: parameter on ", p.device(), "; this build has no CPU path");
+            TORCH_CHECK(p.is_cuda(), "FusedAdamW: parameter on ", p.device(), "; there is no CPU path");
             py::object st = py::reinterpret_borrow<py::object>(item(state.ptr(), p_));
             if (!st || PyObject_Size(st.ptr()) == 0) {
                 st = optimizer.attr("_new_state")(py::handle(p_), group_);
