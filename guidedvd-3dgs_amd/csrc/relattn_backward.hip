@@ -11,6 +11,8 @@
 //   k_rel_dkv     a wave = 32 keys; walks the queries; dS of the table from the corrected delta: by distance into an array of the wave's own in LDS, blocks beyond
 //                 the last border into one register; at the end distances are summed into buckets, one row of partial sums a workgroup
 //   k_rel_table   sums the partial rows, 64 bits
+// P and dS are rounded to the inputs' 16 bits as operands of the second products, the only type the matrix unit takes at this rate: 2^-8 (bf16) or 2^-11 (fp16) of each at most, which sums of
+// many terms average; the table is summed from dS in 32 bits.
 // Bound by instruction issue (two waves a SIMD, 200 registers): 2304 rows, 10 heads, 180 workgroups: 43 and 53 us; 9216 rows, 5 heads: 282 and 340 us, 770 and 640 TFLOP/s of 4
 // products each.
 // Up to 32 queries and keys: k_rel_short_bwd, a wave an item as in the forward; the wave's head is fixed, so dS is summed over its items in registers and goes

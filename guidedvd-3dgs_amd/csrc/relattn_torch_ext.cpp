@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <ATen/hip/EmptyTensor.h>
@@ -201,11 +202,19 @@ at::Tensor differentiable(const at::Tensor& q_, const at::Tensor& k_, const at::
 
 #define GVD_WANT(cond, ...) TORCH_CHECK_VALUE(cond, "relative_bias_attention: ", __VA_ARGS__)
 
-// q, k, v: 16-bit, on one device, heads of 64 (the caller has looked).
-at::Tensor attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Tensor& table_, int64_t heads, const at::Tensor& first, bool both, bool causal, int64_t q_start,
-                  const c10::optional<at::Tensor>& q_starts_, const c10::optional<at::Tensor>& kv_lens_, double scale, bool frame_major)
+// Nothing where the kernels do not cover the call (types, head dim) or a number is out of range: the caller looks closer.
+c10::optional<at::Tensor> attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Tensor& table_, int64_t heads, const at::Tensor& first, bool both, bool causal,
+                                 const py::object& start, const c10::optional<at::Tensor>& kv_lens_, const c10::optional<double>& scale_, bool frame_major)
 {
-    const at::Tensor q_starts = q_starts_.value_or(at::Tensor()), kv_lens = kv_lens_.value_or(at::Tensor());
+    at::Tensor q_starts;
+    int64_t q_start = 0;
+    if (THPVariable_Check(start.ptr())) q_starts = THPVariable_Unpack(start.ptr());
+    else q_start = start.cast<int64_t>();
+    const at::Tensor kv_lens = kv_lens_.value_or(at::Tensor());
+    const double scale = scale_.value_or(0.125);
+    if (!q.is_cuda() || (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
+        heads <= 0 || q.dim() != 3 || q.size(2) != heads * 64 || !(scale > 1e-30 && scale < 1e30) || q_start < -(1 << 29) || q_start > 1 << 29)
+        return c10::nullopt;
     const Config c = {first, kv_lens, heads, q_start, both, causal, frame_major, scale};
     const int bd = c.batch_dim();
     GVD_WANT(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes(), "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), ": three dimensions each, k and v of one shape");
@@ -217,7 +226,7 @@ at::Tensor attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Ten
              "table ", table_.scalar_type(), " ", table_.sizes(), ": [buckets, heads] of float32, float16 or bfloat16, an even number of buckets where both directions have "
              "their own");
     for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&k, &v, &table_}) GVD_WANT(t->device() == q.device(), t == &k ? "k" : t == &v ? "v" : "table", " is on ", t->device(), ", q on ", q.device());
-    for (const at::Tensor* t : {&q_starts, &kv_lens})
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q_starts, &kv_lens})
         GVD_WANT(!t->defined() || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->device() == q.device() && t->is_contiguous()),
                  t == &kv_lens ? "kv_lens" : "q_start", ": ", t->scalar_type(), " ", t->sizes(), " on ", t->device(), "; a contiguous int32 [", B, "] on ", q.device(), " is wanted");
     const at::Tensor table = table_.contiguous();

@@ -410,6 +410,9 @@ def attention(q, k, v, heads, frame_major=False, accum=None, accum_scale=1.0):
     return o if accum is None else accum + accum_scale * o
 
 
+_relative = None     # (the module that imports this one)
+
+
 def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirectional=True, causal=False, q_start=0, kv_lens=None, scale=None,
                             frame_major=False):
     """Attention with a learned bias by relative position: softmax_j(scale q_i . k_j + table[bucket(j - (q_start + i)), h]) v_j per head.
@@ -422,9 +425,12 @@ def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirect
     causal: keys j <= q_start + i only.  q_start: position of query 0 among the keys, a number, or (inference) int32 [B]: new tokens against a cache.
     kv_lens int32 [B]: keys and values at and behind it are not seen, whatever they hold (their gradients are zeros); 0 is a length.  Rows of k and v before it
         have to be finite also where causal hides them from some queries.
-    A query that sees nothing gives zeros and has no gradient.  scale: default 64 ** -0.5."""
-    from . import relative
-    return relative.relative_bias_attention(q, k, v, table, heads, max_distance=max_distance, bidirectional=bidirectional, causal=causal, q_start=q_start,
+    A query that sees nothing gives zeros and has no gradient.  scale: default 64 ** -0.5.  Weights and their gradients pass through the inputs' 16 bits on their way into
+        the second products: in fp16 scale a loss whose gradients are small, as for any fp16 backward.  First derivatives only."""
+    global _relative
+    if _relative is None:
+        from . import relative as _relative
+    return _relative.relative_bias_attention(q, k, v, table, heads, max_distance=max_distance, bidirectional=bidirectional, causal=causal, q_start=q_start,
                                             kv_lens=kv_lens, scale=scale, frame_major=frame_major)
 
 

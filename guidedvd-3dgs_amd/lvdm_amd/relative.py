@@ -136,13 +136,13 @@ def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirect
                             frame_major=False):
     """See ops.relative_bias_attention."""
     on_dev = ops._require_device(q, "relative_bias_attention")
+    if on_dev:
+        buckets = table.shape[0]
+        out = (_EXT or ext()).attend(q, k, v, table, heads, _first_tensor(buckets // 2 if bidirectional else buckets, max_distance), bidirectional, causal, q_start,
+                                     kv_lens, scale, frame_major)
+        if out is not None:
+            return out
     scale = (q.shape[-1] // max(heads, 1)) ** -0.5 if scale is None else float(scale)
-    starts = torch.is_tensor(q_start)
-    if (on_dev and q.dtype in (torch.float16, torch.bfloat16) and k.dtype is q.dtype and v.dtype is q.dtype and heads > 0 and q.shape[-1] == heads * 64
-            and 1e-30 < scale < 1e30 and (starts or -2 ** 29 <= q_start <= 2 ** 29)):
-        side = table.shape[0] // 2 if bidirectional else table.shape[0]
-        return ext().attend(q, k, v, table, heads, _first_tensor(side, max_distance), bidirectional, causal, 0 if starts else q_start, q_start if starts else None,
-                            kv_lens, scale, frame_major)
     _check_arguments(q, k, v, table, heads, bidirectional, q_start, kv_lens, scale, frame_major, max_distance)
     if on_dev:
         ops._torch_form("relative_bias_attention", f"dtypes {q.dtype}, {k.dtype}, {v.dtype}, head dim {q.shape[-1] // heads} (the MFMA kernels cover 16-bit heads of 64)")
