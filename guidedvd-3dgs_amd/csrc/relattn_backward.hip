@@ -4,7 +4,7 @@
 //     dQ = scale dS K,  dK = scale dS^T Q,  dT[b, h] = sum of dS_ij over the (i, j) whose distance lies in bucket b
 //
 // General rows, kernels in turn, no sum whose order could change:
-//   k_rel_dq      a wave = 32 queries; walks the keys with delta from dO . O.  O was rounded, and so were the P that made it, so this delta is 2^-9 |dO| |O| off
+//   k_rel_dq      a wave = 32 queries; walks the keys with delta from dO . O.  O was rounded, and so were the P that made it, so this delta is up to 2^-8 |dO| |O| off
 //                 (bf16), which is much where V has a mean (dS is a difference then) and for a table's gradient in 32 bits (its sums cancel: a row's dS
 //                 sums to 0).  But a row's dS as formed sums to exactly what delta was off by, so dQ = dS K - (that sum) P K, one more product on K's
 //                 fragments, and the delta that the kernel leaves for k_rel_dkv is right.  (V = noise + 3, bf16: dQ 2.1 % off without, 0.24 % with)
