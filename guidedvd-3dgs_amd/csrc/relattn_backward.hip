@@ -459,22 +459,26 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
     float L_next;
     int len_next;
     auto load_kv = [&](int b) {
+        int row_ = row;
+        asm volatile("" : "+v"(row_));   // (not kept from item to item: the registers are full)
         len_next = len_of(g, b);
         const int last = len_next > 0 ? len_next - 1 : 0;
         const size_t kv = (size_t)b * g.kv_bs + (size_t)h * 64 + c8;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = 8 * i + row;
+            const int r = 8 * i + row_;
             const size_t j = r < last ? r : last;
             rk[i] = *reinterpret_cast<const vec8*>(k + kv + j * (size_t)g.kv_rs);
             rv[i] = *reinterpret_cast<const vec8*>(v + kv + j * (size_t)g.kv_rs);
         }
     };
     auto load_q = [&](int b) {
+        int row_ = row;
+        asm volatile("" : "+v"(row_));   // (not kept from item to item: the registers are full)
         const size_t qb = (size_t)b * g.q_bs + (size_t)h * 64 + c8, gb = (size_t)b * g.o_bs + (size_t)h * 64 + c8;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = 8 * i + row;
+            const int r = 8 * i + row_;
             const size_t n = r < g.Nq ? r : g.Nq - 1;
             rq[i] = *reinterpret_cast<const vec8*>(q + qb + n * (size_t)g.q_rs);
             rg[i] = *reinterpret_cast<const vec8*>(d_o + gb + n * (size_t)g.o_rs);
@@ -483,11 +487,13 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
     };
     auto operand = [&](const T (&x)[32][OP], int ks) { return *reinterpret_cast<const vec8*>(&x[r32][16 * ks + 8 * hi]); };
     auto store_rows = [&](const f16v& x0, const f16v& x1, float mul, T* base, size_t rstride, int nrows) {
+        int row_ = row;
+        asm volatile("" : "+v"(row_));   // (not kept from item to item: the registers are full)
         store_row<T>(&sV[wave][r32][0], x0, x1, mul, hi);
         wave_order();
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = 8 * i + row;
+            const int r = 8 * i + row_;
             const u4 w = *reinterpret_cast<const u4*>(&sV[wave][r][c8]);
             if (r < nrows) __builtin_nontemporal_store(w, reinterpret_cast<u4*>(base + (size_t)r * rstride + c8));
         }
