@@ -76,28 +76,33 @@ namespace {
 
 // ---- general rows ------------------------------------------------------------------------------------------------------------
 // The vector unit bounds this kernel: 32 exponentials a lane, query block and tile, against 16 products of the matrix unit.  9216 rows, 5 heads: 147 us, 740 TFLOP/s; 20 heads
-// 540, 805; 2304 rows, 10 heads: 37.  So the loop does little else:
+// 540, 805; 2304 rows, 10 heads: 31.7.  So the loop does little else:
 //   * the maximum is not looked for: weights are formed with the running one, and a row sum above 2^15 (always for the first tile: the maximum starts
 //     below every score) sends the block through the exact path.  Numerators and denominator share the maximum, so any one that keeps weights finite
 //     gives the exact softmax;
 //   * each half wave keeps its own row sum, of the rounded weights (one dot product for two), or, where the backward will build on it (LSE), of the unrounded
 //     ones: its weights sum to 1 in 32 bits then, which the table's gradient needs; the halves meet at the end;
 //   * a block whose distances share one bias adds it to the exponent's shift, and its products start from the matrix unit's own zero.
-template <typename T, int QB, bool PART, bool LSE>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+//   * KS = 2: eight waves, two a SIMD where the grid gives a CU one workgroup only; the second four take every other tile of keys for the same rows and hand
+//     maximum, sum and result over through LDS at the end.
+template <typename T, int QB, bool PART, bool LSE, int KS>
+__global__ void __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2)))
 k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
           float* __restrict__ part_o, float2* __restrict__ part_ml, int parts)
 {
     typedef typename Tr<T>::vec8 vec8;
-    __shared__ __attribute__((aligned(16))) T sKb[2][KV_TILE][LDS_ROW];
-    __shared__ __attribute__((aligned(16))) T sVb[2][KV_TILE][LDS_ROW];
+    constexpr int STAGE = KS * KV_TILE;   // keys between two barriers
+    __shared__ __attribute__((aligned(16))) T sKb[2][STAGE][LDS_ROW];
+    __shared__ __attribute__((aligned(16))) T sVb[2][STAGE][LDS_ROW];
+    static_assert(KS == 1 || sizeof(sKb) + sizeof(sVb) >= 4 * QB * 34 * 64 * sizeof(float), "the hand-over uses the tiles' memory");
     extern __shared__ __attribute__((aligned(16))) float sBias[];
 
     int bh, tile_y;
     xcd_item_tile(bh, tile_y);
     const int qtile = PART ? tile_y / parts : tile_y, part = PART ? tile_y - qtile * parts : 0;
     const int b = bh / g.H, h = bh - b * g.H;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave8 = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wave8 & 3, hi = lane >> 5, col = lane & 31;
+    const int k_off = KS == 1 ? 0 : KV_TILE * (wave8 >> 2);   // the wave's tile of a stage
     const int start = start_of(g, b), len = len_of(g, b);
     const T* qb = q + (size_t)b * g.q_bs + (size_t)h * 64;
     const T* kb = k + (size_t)b * g.kv_bs + (size_t)h * 64;
@@ -107,7 +112,7 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     int k_lo = 0, k_hi = g.causal ? clamp_int(start + q_last + 1, 0, len) : len;
     const int k_full = g.causal ? clamp_int(start + q0 + 1, 0, len) : len;
     if (PART) {
-        const int per = ((k_hi + KV_TILE - 1) / KV_TILE + parts - 1) / parts * KV_TILE;
+        const int per = ((k_hi + STAGE - 1) / STAGE + parts - 1) / parts * STAGE;
         k_lo = part * per < k_hi ? part * per : k_hi;
         k_hi = k_lo + per < k_hi ? k_lo + per : k_hi;
     }
@@ -132,10 +137,10 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     // meets a weight of 0): only the last tile looks.
     vec8 rk[2], rv[2];
     const int row = tid >> 3, c8 = (tid & 7) * 8;
-    const size_t lane_off = (size_t)row * (size_t)g.kv_rs + c8, half_off = 32 * (size_t)g.kv_rs;
+    const size_t lane_off = (size_t)row * (size_t)g.kv_rs + c8, half_off = 32 * KS * (size_t)g.kv_rs;
     auto prefetch = [&](int kt) {
         const size_t base = (size_t)kt * (size_t)g.kv_rs;
-        if (kt + KV_TILE <= len) {
+        if (kt + STAGE <= len) {
 #pragma unroll
             for (int ps = 0; ps < 2; ps++) {
                 rk[ps] = *reinterpret_cast<const vec8*>(kb + base + (lane_off + ps * half_off));
@@ -144,7 +149,7 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         } else {
 #pragma unroll
             for (int ps = 0; ps < 2; ps++) {
-                const int key = kt + row + 32 * ps;
+                const int key = kt + row + 32 * KS * ps;
                 const size_t off = (size_t)(key < len ? key : len - 1) * (size_t)g.kv_rs + c8;
                 rk[ps] = *reinterpret_cast<const vec8*>(kb + off);
                 rv[ps] = *reinterpret_cast<const vec8*>(vb + off);
@@ -155,21 +160,22 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     auto commit = [&](int buf) {
 #pragma unroll
         for (int ps = 0; ps < 2; ps++) {
-            *reinterpret_cast<vec8*>(&sKb[buf][row + 32 * ps][c8]) = rk[ps];
-            *reinterpret_cast<vec8*>(&sVb[buf][row + 32 * ps][c8]) = rv[ps];
+            *reinterpret_cast<vec8*>(&sKb[buf][row + 32 * KS * ps][c8]) = rk[ps];
+            *reinterpret_cast<vec8*>(&sVb[buf][row + 32 * KS * ps][c8]) = rv[ps];
         }
     };
     if (k_lo < k_hi) prefetch(k_lo);
-    fill_bias(g, h, sBias, tid, 256);
+    fill_bias(g, h, sBias, tid, 256 * KS);
     float far_past = 0.f, far_ahead = 0.f;
 
-    auto tile = [&](int kt, int buf, auto masked_tag) {
+    auto tile = [&](int stage, int buf, auto masked_tag) {
         constexpr bool MASKED = decltype(masked_tag)::value;
-        if (kt + KV_TILE < k_hi) {
+        if (stage + STAGE < k_hi) {
             commit(buf ^ 1);
-            if (kt + 2 * KV_TILE < k_hi) prefetch(kt + 2 * KV_TILE);
+            if (stage + 2 * STAGE < k_hi) prefetch(stage + 2 * STAGE);
         }
-        const T (*sK)[LDS_ROW] = sKb[buf];
+        const int kt = stage + k_off;
+        const T (*sK)[LDS_ROW] = sKb[buf] + k_off;
         f16v s0[QB], s1[QB];
         float far[QB];   // the single bias of a far block, in the exponent
         vec8 a0[4], a1[4];
@@ -248,8 +254,8 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
         for (int kbk = 0; kbk < 2; kbk++)
 #pragma unroll
             for (int k2 = 0; k2 < 2; k2++) {
-                const vec8 v0 = transposed_operand(&sVb[buf][0][0], LDS_ROW, 32 * kbk + 16 * k2, 0, lane);
-                const vec8 v1 = transposed_operand(&sVb[buf][0][0], LDS_ROW, 32 * kbk + 16 * k2, 32, lane);
+                const vec8 v0 = transposed_operand(&sVb[buf][0][0], LDS_ROW, k_off + 32 * kbk + 16 * k2, 0, lane);
+                const vec8 v1 = transposed_operand(&sVb[buf][0][0], LDS_ROW, k_off + 32 * kbk + 16 * k2, 32, lane);
 #pragma unroll
                 for (int qi = 0; qi < QB; qi++) {
                     const vec8 pf = packed_operand<T>(kbk == 0 ? pk0[qi] : pk1[qi], k2);
@@ -262,16 +268,43 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
 
     if (k_lo < k_hi) {   // (uniform over the workgroup)
         commit(0);
-        if (k_lo + KV_TILE < k_hi) prefetch(k_lo + KV_TILE);
+        if (k_lo + STAGE < k_hi) prefetch(k_lo + STAGE);
         __syncthreads();
         far_past = sBias[0] * g.c;
         far_ahead = sBias[bias_len(g.reach) - 1] * g.c;
         int kt = k_lo, buf = 0;
-        for (; kt < k_hi && kt + KV_TILE <= k_full; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::false_type{});
-        for (; kt < k_hi; kt += KV_TILE, buf ^= 1) tile(kt, buf, std::true_type{});
+        for (; kt < k_hi && kt + STAGE <= k_full; kt += STAGE, buf ^= 1) tile(kt, buf, std::false_type{});
+        for (; kt < k_hi; kt += STAGE, buf ^= 1) tile(kt, buf, std::true_type{});
     }
 #pragma unroll
     for (int qi = 0; qi < QB; qi++) l[qi] += __shfl_xor(l[qi], 32, 64);
+    if (KS == 2) {   // (the loop's last barrier lies behind all reads of the tiles)
+        auto at = [&](int qi) { float* base = reinterpret_cast<float*>(qi % 2 ? &sVb[0][0][0] : &sKb[0][0][0]); return base + (wave * 34) * 64 + lane; };
+        if (wave8 >= 4) {
+#pragma unroll
+            for (int qi = 0; qi < QB; qi++) {
+                float* x = at(qi);
+#pragma unroll
+                for (int r = 0; r < 16; r++) { x[64 * r] = o0[qi][r]; x[64 * (16 + r)] = o1[qi][r]; }
+                x[64 * 32] = m[qi];
+                x[64 * 33] = l[qi];
+            }
+        }
+        __syncthreads();
+        if (wave8 >= 4) return;
+#pragma unroll
+        for (int qi = 0; qi < QB; qi++) {
+            const float* x = at(qi);
+            const float m1 = x[64 * 32], top = fmaxf(m[qi], m1), w0 = __builtin_amdgcn_exp2f(m[qi] - top), w1 = __builtin_amdgcn_exp2f(m1 - top);
+            m[qi] = top;
+            l[qi] = l[qi] * w0 + x[64 * 33] * w1;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                o0[qi][r] = o0[qi][r] * w0 + x[64 * r] * w1;
+                o1[qi][r] = o1[qi][r] * w0 + x[64 * (16 + r)] * w1;
+            }
+        }
+    }
 #pragma unroll
     for (int qi = 0; qi < QB; qi++) {
         if (query[qi] >= g.Nq) continue;
@@ -609,25 +642,26 @@ __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restric
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 enum Form { SHORT, FEW, GENERAL };
 
-struct Plan { Form form; int qb, tiles, parts; };
+struct Plan { Form form; int qb, tiles, parts, ks; };
 
 // Which kernel, how many query blocks a wave, and into how many parts the keys are cut.
 // General rows: what a choice takes is estimated, in microseconds, and the least is taken.  A workgroup of 128 rows takes 0.95 a tile alone on its CU and 0.745 with
-// others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products); a round of workgroups starts with 4 (bias, first tiles); parts
+// others, one of 256 rows 1.5 and 1.3 (their K and V fragments serve twice the products), one of 128 rows and eight waves 1.48 for two tiles, alone (with others there it has
+// nothing to gain: 2304, 20 heads 61.5 against 58); a round of workgroups starts with 4 (bias, first tiles), with eight waves 5; parts
 // take 8 (their stores, the join's launch) and 3.3e-5 a row and part.  Measured, with the join (us): 9216 queries and keys, 5 heads: 128 rows 212, in 2 parts 162; 256 rows 212, in 2 parts
-// 186, in 4 parts 157.  2304, 10 heads: 128 rows 37, 256 rows 55, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 41, in 2 parts 53; 256 rows 48.  Over ten
+// 186, in 4 parts 157.  2304, 10 heads: 128 rows 37, with eight waves 31.7, 256 rows 55, 128 rows in 2 parts 42.  1024, 80 items: 128 rows 41, in 2 parts 53; 256 rows 48.  Over ten
 // shapes and eight choices each, what it picks is 0.5 % off the best on average, 3 % at most.
 Plan plan_of(const Geo& g, int B, int cus)
 {
     const long long bh = (long long)B * g.H;
-    if (g.Nq <= 32 && g.Nk <= 32) return { SHORT, 1, 1, 1 };
+    if (g.Nq <= 32 && g.Nk <= 32) return { SHORT, 1, 1, 1, 1 };
     if (g.Nq <= 4) {   // few rows: 4 workgroups a CU, at least 256 keys each
         long long parts = ((long long)cus * 4 + bh - 1) / bh;
         const long long most = (g.Nk + 255) / 256;
         if (parts > most) parts = most;
-        return { FEW, 1, 1, (int)(parts < 64 ? parts : 64) };
+        return { FEW, 1, 1, (int)(parts < 64 ? parts : 64), 1 };
     }
-    Plan best = { GENERAL, 1, 1, 1 };
+    Plan best = { GENERAL, 1, 1, 1, 1 };
     double least = 1e30;
     const int tiles = (g.Nk + KV_TILE - 1) / KV_TILE;
     for (int qb = 1; qb <= 2; qb++) {
@@ -636,7 +670,11 @@ Plan plan_of(const Geo& g, int B, int cus)
             const double load = (double)bh * qtiles * parts / cus, rounds = load <= 1.0 ? 1.0 : (load < 8.0 ? __builtin_ceil(load) : load);
             const double a_tile = rounds == 1.0 ? (qb == 2 ? 1.5 : 0.95) : rounds * (qb == 2 ? 1.3 : 0.745);
             const double t = 4.0 * rounds + (tiles + parts - 1) / parts * a_tile + (parts > 1 ? 8.0 + 3.3e-5 * (double)bh * g.Nq * parts : 0.0);
-            if (t < least) { least = t; best = { GENERAL, qb, qtiles, parts }; }
+            if (t < least) { least = t; best = { GENERAL, qb, qtiles, parts, 1 }; }
+            if (qb == 2 || rounds > 1.0) continue;
+            const int stages = (tiles + 1) / 2;   // of 128 keys
+            const double t2 = 5.0 + (stages + parts - 1) / parts * 1.48 + (t - 4.0 * rounds - (tiles + parts - 1) / parts * a_tile);
+            if (t2 < least) { least = t2; best = { GENERAL, 1, qtiles, parts, 2 }; }
         }
     }
     return best;
@@ -674,12 +712,14 @@ int launch_fwd(const Geo& g, int B, const void* q, const void* k, const void* v,
 #undef GVD_FEW
     } else {
         const dim3 grid((unsigned)BH, (unsigned)(pl.tiles * pl.parts));
-#define GVD_GEN(Q, P) if (lse) GVD_GEN_(Q, P, true); else GVD_GEN_(Q, P, false)
-#define GVD_GEN_(Q, P, L) hipLaunchKernelGGL((k_rel_fwd<T, Q, P, L>), grid, dim3(256), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
-        if (pl.qb == 2 && pl.parts > 1) { GVD_GEN(2, true); }
-        else if (pl.qb == 2) { GVD_GEN(2, false); }
-        else if (pl.parts > 1) { GVD_GEN(1, true); }
-        else { GVD_GEN(1, false); }
+#define GVD_GEN(Q, P, K) if (lse) GVD_GEN_(Q, P, true, K); else GVD_GEN_(Q, P, false, K)
+#define GVD_GEN_(Q, P, L, K) hipLaunchKernelGGL((k_rel_fwd<T, Q, P, L, K>), grid, dim3(256 * K), lds, stream, g, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, po, ml, pl.parts)
+        if (pl.ks == 2 && pl.parts > 1) { GVD_GEN(1, true, 2); }
+        else if (pl.ks == 2) { GVD_GEN(1, false, 2); }
+        else if (pl.qb == 2 && pl.parts > 1) { GVD_GEN(2, true, 1); }
+        else if (pl.qb == 2) { GVD_GEN(2, false, 1); }
+        else if (pl.parts > 1) { GVD_GEN(1, true, 1); }
+        else { GVD_GEN(1, false, 1); }
 #undef GVD_GEN
 #undef GVD_GEN_
     }
