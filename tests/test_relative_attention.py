@@ -293,6 +293,17 @@ def test_keys_in_parts(nq, nk):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,nq,nk", [(2, 3, 140, 200), (1, 2, 300, 700), (1, 2, 70, 1100), (1, 5, 333, 3001), (3, 8, 129, 1001), (8, 20, 130, 75), (1, 20, 5, 4000)])
+def test_every_division_of_the_work(B, H, nq, nk, dtype):
+    """128 or 256 rows a workgroup, four waves or eight, the keys whole or in parts: with and without what the backward keeps, whole and ragged, causal from the middle."""
+    q, k, v, t, g = inputs(B, H, nq, nk, dtype, seed=nq)
+    check(q, k, v, t, g, H)
+    lens = torch.tensor([nk - 1, nk // 2, 1, 0, nk, 64, 65, 2][:B], dtype=torch.int32, device=DEV)
+    check(q, k, v, t, g, H, causal=True, q_start=nk // 2, kv_lens=lens)
+
+
+@gpu
 def test_a_table_of_32_bits_has_a_gradient_of_32_bits():
     """Sums that cancel: with delta from the rounded output the error would be about 2^-10; independent errors of 32 bits leave below 1e-5 of the norm."""
     for kw, shape in ((dict(), (1, 4, 500, 500)), (dict(causal=True), (2, 2, 301, 301)), (dict(frame_major=True), (300, 4, 25, 25))):
