@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
@@ -178,8 +179,6 @@ void refuse_foreign_accumulators(std::initializer_list<const at::Tensor*> inputs
 
 at::Tensor differentiable(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& table, const Config& c)
 {
-    for (const at::Tensor* t : {&q_, &k_, &v_, &table})
-        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "relative_bias_attention: no forward-mode derivatives");
     const std::shared_ptr<RelativeBiasAttentionBackward> node(new RelativeBiasAttentionBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(q_, k_, v_, table));
     at::Tensor out;
@@ -215,6 +214,10 @@ c10::optional<at::Tensor> attend(const at::Tensor& q, at::Tensor k, at::Tensor v
     if (!q.is_cuda() || (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
         heads <= 0 || q.dim() != 3 || q.size(2) != heads * 64 || !(scale > 1e-30 && scale < 1e30) || q_start < -(1 << 29) || q_start > 1 << 29)
         return c10::nullopt;
+    // a tangent needs no requires_grad and outlives no_grad(): looked for in every call, also in those that keep nothing for a backward
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &k, &v, &table_})
+            TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "relative_bias_attention: no forward-mode derivatives");
     const Config c = {first, kv_lens, heads, q_start, both, causal, frame_major, scale};
     const int bd = c.batch_dim();
     GVD_WANT(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes(), "q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), ": three dimensions each, k and v of one shape");
