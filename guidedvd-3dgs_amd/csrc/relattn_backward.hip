@@ -10,7 +10,7 @@
 //                 fragments, and the delta that the kernel leaves for k_rel_dkv is right.  (V = noise + 3, bf16: dQ 2.1 % off without, 0.24 % with)
 //   k_rel_dkv     a wave = 32 keys; walks the queries; dS of the table from the corrected delta: by distance into an array of the wave's own in LDS, blocks beyond
 //                 the last border into one register; at the end distances are summed into buckets, one row of partial sums a workgroup
-//   k_rel_table   sums the partial rows, 64 bits
+//   k_rel_table   sums the partial rows, 64 bits; an entry that masks or that counts as another value has no gradient
 // P and dS are rounded to the inputs' 16 bits as operands of the second products, the only type the matrix unit takes at this rate: 2^-8 (bf16) or 2^-11 (fp16) of each at most, which sums of
 // many terms average; the table is summed from dS in 32 bits.
 // Bound by instruction issue (two waves a SIMD, 200 registers): 2304 rows, 10 heads, 180 workgroups: 43 and 53 us; 9216 rows, 5 heads: 282 and 340 us, 770 and 640 TFLOP/s of 4
@@ -407,7 +407,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
 
 // Partial rows j = 0 .. count - 1 of head h lie at row ((j / tiles) H + h) tiles + j % tiles.  A wave a table entry, 64 bits, fixed order.
 template <typename E>
-__global__ void __launch_bounds__(64) k_rel_table(const float* __restrict__ part, E* __restrict__ dtable, int H, int buckets, int tiles, int count)
+__global__ void __launch_bounds__(64) k_rel_table(const float* __restrict__ part, const E* __restrict__ table, E* __restrict__ dtable, int H, int buckets, int tiles, int count)
 {
     const int bucket = blockIdx.x, h = blockIdx.y;
     double x = 0.0;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(64) k_rel_table(const float* __restrict__ part
     }
 #pragma unroll
     for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w, 64);
-    if (threadIdx.x == 0) dtable[bucket * H + h] = (E)(float)x;
+    if (threadIdx.x == 0) dtable[bucket * H + h] = without_gradient((float)table[bucket * H + h]) ? (E)0.f : (E)(float)x;
 }
 
 // ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
@@ -658,7 +658,7 @@ int launch_bwd(const Geo& g, int B, const void* q, const void* k, const void* v,
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(-2, "launch k_rel_*_bwd", e);
     const dim3 grid((unsigned)g.buckets, (unsigned)g.H);
-#define GVD_TABLE(E) hipLaunchKernelGGL(k_rel_table<E>, grid, dim3(64), 0, stream, (const float*)part, (E*)dtable, g.H, g.buckets, tiles, count)
+#define GVD_TABLE(E) hipLaunchKernelGGL(k_rel_table<E>, grid, dim3(64), 0, stream, (const float*)part, (const E*)g.table, (E*)dtable, g.H, g.buckets, tiles, count)
     if (g.table_type == 0) GVD_TABLE(float); else if (g.table_type == 1) GVD_TABLE(_Float16); else GVD_TABLE(__bf16);
 #undef GVD_TABLE
     e = hipGetLastError();

@@ -47,10 +47,14 @@ __device__ __forceinline__ float table_at(const Geo& g, int bucket, int h)
 // The bias as the products' accumulators start from it: over the scale, so that scores come out of the matrix unit as (q.k + bias / scale).  Entries at or below
 // -10000 mask their bucket, as -infinity does: among them are the lowest values of every type and the constants used in their place, and a score that
 // far out would leave 32 bits nothing for q.k.  For the same reason an entry counts as 10000 at most.
+constexpr float MASKS_AT = -10000.f, MOST = 10000.f;
 __device__ __forceinline__ float start_value(const Geo& g, float bias)
 {
-    return (bias <= -10000.f ? -INFINITY : (bias > 10000.f ? 10000.f : bias)) * g.inv_scale;
+    return (bias <= MASKS_AT ? -INFINITY : (bias > MOST ? MOST : bias)) * g.inv_scale;
 }
+
+// Whether results do not depend on an entry: where it masks its bucket, and where another value counts in its place.
+__device__ __forceinline__ bool without_gradient(float bias) { return bias <= MASKS_AT || bias > MOST; }
 
 // MIRRORED: descending distances, for blocks whose registers run over queries.
 template <bool MIRRORED = false>

@@ -421,7 +421,7 @@ def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirect
     table [buckets, heads], float32, fp16 or bf16; gradients of q, k, v and table (no atomics across workgroups: the same call gives the same bits).
     bucket(d): the first half of a side's buckets hold one distance each, the others equal ratios up to max_distance, the last everything beyond;
         bidirectional: keys ahead (d > 0) have the table's upper half; otherwise they share bucket 0 (`relative.relative_buckets`).
-        An entry at or below -10000 (-infinity, a type's lowest value) masks its bucket; one above 10000 counts as 10000.
+        An entry at or below -10000 (-infinity, a type's lowest value) masks its bucket; one above 10000 counts as 10000.  Neither has a gradient.
     causal: keys j <= q_start + i only.  q_start: position of query 0 among the keys, a number, or (inference) int32 [B]: new tokens against a cache.
     kv_lens int32 [B]: keys and values at and behind it are not seen, whatever they hold (their gradients are zeros); 0 is a length.  Rows of k and v before it
         have to be finite also where causal hides them from some queries.

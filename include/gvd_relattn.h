@@ -8,7 +8,7 @@
  *     s_ij = scale q_i . k_j + table[bucket(j - (start_b + i)), h],   seen: j < len_b, and j <= start_b + i where causal
  *     out_i = sum_j softmax_j(s_ij) v_j;  zeros where i sees nothing
  *
- * A table entry at or below -10000 masks its bucket: i does not see j there, and the entry has no gradient.  An entry above 10000 counts as 10000.
+ * A table entry at or below -10000 masks its bucket: i does not see j there.  An entry above 10000 counts as 10000.  Neither has a gradient.
  *
  * bucket(d) of a distance d: side = both ? buckets / 2 : buckets; n = both ? |d| : max(-d, 0); the last k < side with first[k] <= n, plus side where
  * both and d > 0.  Keys and values behind len_b are not read into any result.

@@ -17,6 +17,85 @@ def inputs(B, H, Nq, Nk, dtype=torch.float16, table_dtype=torch.float32, buckets
     return mk(Nq), mk(Nk), mk(Nk), (0.8 * torch.randn(buckets, H, generator=gen)).to(table_dtype).to(DEV), mk(Nq)
 
 
+def formula(q, k, v, t, H, g, d32, **kw):
+    """Results in 64 bits, by the explicit form and autograd, and how far a kernel may be: d32 is the relative error of a weight before it is rounded; weights and dS are
+    rounded to the rows' type (u), results once more.  dS = P (dP - delta): each factor d32 off, delta as a sum of weights times dP, and dQ forms it from a delta that the
+    rounded output gave and takes the difference off again (2 u of a row's sum of P |dP| at most)."""
+    u, u_t = torch.finfo(q.dtype).eps / 2, torch.finfo(t.dtype).eps / 2
+    small = 2.0 ** -24 if q.dtype == torch.float16 else 2.0 ** -126
+    leaves = [x.detach().double().requires_grad_(True) for x in (q, k, v, t)]
+    out = relative.relative_bias_attention_math(*leaves, H, **kw)
+    want = dict(zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *torch.autograd.grad(out, leaves, g.double()))))
+    scale = kw.get("scale") or D ** -0.5
+    heads = lambda x: x.detach().double().reshape(*x.shape[:2], H, D).transpose(1, 2)  # noqa: E731
+    rows = lambda x: x.transpose(1, 2).reshape(x.shape[0], x.shape[2], H * D)  # noqa: E731
+    Q, K, V, G = (heads(x) for x in (q, k, v, g))
+    dist = torch.arange(K.shape[2], device=DEV)[None] - torch.arange(Q.shape[2], device=DEV)[:, None]
+    bucket = relative.relative_buckets(dist, t.shape[0], kw.get("max_distance", 128), kw.get("bidirectional", True))
+    T = t.detach().double().clamp(max=10000.0)
+    a = Q @ K.transpose(-1, -2) * scale + T.masked_fill(T <= -10000.0, float("-inf"))[bucket].permute(2, 0, 1)
+    if kw.get("causal"):
+        a = a.masked_fill(dist > 0, float("-inf"))
+    p = a.softmax(-1)
+    dp = G @ V.transpose(-1, -2)
+    spread = (p * dp.abs()).sum(-1, keepdim=True)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    e_p = (u + d32) * p + small
+    e_ds = u * ds.abs() + 2 * u * u * p * spread * 4 + 3 * d32 * p * (dp.abs() + spread) + small
+    e_t = torch.zeros_like(want["dtable"]).index_add_(0, bucket.reshape(-1), (3 * d32 * p * (dp.abs() + spread)).sum(0).permute(1, 2, 0).reshape(-1, H))
+    err = dict(out=rows(e_p @ V.abs()), dq=rows(e_ds @ K.abs()) * scale, dk=rows(e_ds.transpose(-1, -2) @ Q.abs()) * scale, dv=rows(e_p.transpose(-1, -2) @ G.abs()), dtable=e_t)
+    return want, {n: 1.01 * e + (u_t if n == "dtable" else u) * want[n].abs() + 2.0 ** -24 for n, e in err.items()}
+
+
+def kernels(q, k, v, t, H, g, **kw):
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v, t)]
+    out = ops.relative_bias_attention(*leaves, H, **kw)
+    return dict(zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *torch.autograd.grad(out, leaves, g))))
+
+
+def close(got, want, err):
+    for n, y in want.items():
+        off = (got[n].double() - y).abs()
+        assert bool((off <= err[n]).all()), (n, float((off / err[n]).max()))
+
+
+# ---- entries that are brought to a limit -----------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("n", [25, 70, 200])
+@pytest.mark.parametrize("table_dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_an_entry_above_the_limit_counts_as_the_limit_and_has_no_gradient(table_dtype, n):
+    """Scores start from 10000 / scale = 80000, whose half step is 2^-8: 64 additions leave a score at most 64 x 2^-8 / 8 = 2^-5 off, a weight (over a sum of
+    weights) exp(2^-4) - 1 < 0.065."""
+    H = 2
+    q, k, v, t, g = inputs(2, H, n, n, table_dtype=table_dtype, seed=n)
+    for entry in (1e4, 2e4, 6e4, float("inf")):
+        t[3], t[6] = entry, entry                 # keys three and six behind: the softmax is between the two
+        if table_dtype == torch.bfloat16 and entry == 1e4:
+            t[3], t[6] = 9984.0, 9984.0           # (the value below 10000)
+        want, err = formula(q, k, v, t, H, g, 0.065)
+        got = kernels(q, k, v, t, H, g)
+        close(got, want, err)
+        if entry == 1e4:
+            first = got
+            assert bool((want["dtable"][[3, 6]] != 0).all()) and bool((got["dtable"][[3, 6]] != 0).all())     # at the limit itself there is one
+            continue
+        assert bool((want["dtable"][[3, 6]] == 0).all()) and bool((got["dtable"][[3, 6]] == 0).all())
+        if table_dtype != torch.bfloat16:
+            assert all(torch.equal(got[x], first[x]) for x in ("out", "dq", "dk", "dv"))   # whatever the entry: the same results
+
+
+@gpu
+@pytest.mark.parametrize("n", [25, 70])
+def test_an_entry_that_masks_has_no_gradient(n):
+    q, k, v, t, g = inputs(2, 2, n, n, seed=n)
+    for entry in (-1e4, -6e4, float("-inf")):
+        t[3] = entry
+        want, err = formula(q, k, v, t, 2, g, 2.0 ** -15)
+        got = kernels(q, k, v, t, 2, g)
+        close(got, want, err)
+        assert bool((got["dtable"][3] == 0).all()) and bool((got["dtable"][4] != 0).all())
+
+
 # ---- forward-mode derivatives ----------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("n", [1, 25, 70])
