@@ -205,6 +205,8 @@ at::Tensor differentiable(const at::Tensor& q_, const at::Tensor& k_, const at::
 c10::optional<at::Tensor> attend(const at::Tensor& q, at::Tensor k, at::Tensor v, const at::Tensor& table_, int64_t heads, const at::Tensor& first, bool both, bool causal,
                                  const py::object& start, const c10::optional<at::Tensor>& kv_lens_, const c10::optional<double>& scale_, bool frame_major)
 {
+    TORCH_CHECK(first.is_cpu() && first.scalar_type() == at::kInt && first.dim() == 1 && first.numel() > 0 && first.is_contiguous(),
+                "relative_bias_attention: the buckets' first distances are read by the host, as a contiguous int32 row; got ", first.scalar_type(), " ", first.sizes(), " on ", first.device());
     at::Tensor q_starts;
     int64_t q_start = 0;
     if (THPVariable_Check(start.ptr())) q_starts = THPVariable_Unpack(start.ptr());

@@ -67,7 +67,7 @@ def first_distances(side, max_distance):
 
 @functools.lru_cache(maxsize=64)
 def _first_tensor(side, max_distance):
-    return torch.tensor(first_distances(side, max_distance), dtype=torch.int32)
+    return torch.tensor(first_distances(side, max_distance), dtype=torch.int32, device="cpu")     # (kept, and read by the host: whatever the default device is)
 
 
 def relative_buckets(distance, buckets, max_distance=128, bidirectional=True):

@@ -96,6 +96,40 @@ def test_an_entry_that_masks_has_no_gradient(n):
         assert bool((got["dtable"][3] == 0).all()) and bool((got["dtable"][4] != 0).all())
 
 
+# ---- other default devices ---------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def nothing_kept():
+    relative._first_tensor.cache_clear()
+    yield
+    relative._first_tensor.cache_clear()
+
+
+def test_the_first_distances_lie_on_the_host_whatever_the_default_device(nothing_kept):
+    with torch.device("meta"):
+        kept = relative._first_tensor(16, 128)
+    assert kept.device.type == "cpu" and kept.tolist() == list(relative.first_distances(16, 128)) and relative._first_tensor(16, 128) is kept
+
+
+def test_first_distances_that_the_host_cannot_read_are_refused():
+    q, t = torch.zeros(1, 2, D), torch.zeros(8, 1)
+    row = torch.arange(4, dtype=torch.int32)
+    call = lambda first: relative.ext().attend(q, q, q, t, 1, first, True, False, 0, None, None, False)  # noqa: E731
+    assert call(row) is None                            # (rows on the CPU: left to the caller)
+    for first in (row.to("meta"), row.long(), row.view(2, 2), row[::2], row[:0]):
+        with pytest.raises(RuntimeError, match="read by the host"):
+            call(first)
+
+
+@gpu
+def test_a_call_under_another_default_device(nothing_kept):
+    q, k, v, t, g = inputs(2, 2, 25, 25)
+    want = kernels(q, k, v, t, 2, g)
+    relative._first_tensor.cache_clear()
+    with torch.device(DEV):
+        got = kernels(q, k, v, t, 2, g)
+    assert all(torch.equal(got[n], x) for n, x in want.items())
+
+
 # ---- forward-mode derivatives ----------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("n", [1, 25, 70])
