@@ -22,6 +22,7 @@ _LIB_PATH = os.environ.get("GVD_OPTIM_LIB") or os.path.join(os.path.dirname(_HER
 _EXT_PATH = os.path.join(os.path.dirname(_HERE), "lib", "_gvd_optim_torch.so")
 _LIB = _EXT = None
 BLOCK = 256                                 # GVD_ADAMW_BLOCK: elements that share a scale where moments are held in 8 bits
+TINY = 2.0 ** -110                          # a block whose largest magnitude is below this is held as zeros (448 over it would overflow), as in the kernel
 
 
 def lib():
@@ -197,6 +198,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 row[:p.numel()] = _in_order(ordered)
                 row = row.view(-1, BLOCK)
                 big = row.abs().amax(1)
+                big = torch.where(big < TINY, 0.0, big)
                 scales.copy_(big / 448.0)
                 q = torch.where(big[:, None] > 0, row * (448.0 / big[:, None]), 0.0)
                 if codes is st["exp_avg_rms"]:

@@ -1,0 +1,41 @@
+"""FusedAdamW in the calls where it can go wrong without a word: moments at the ends of float32's range, spellings of one memory order, groups that change between steps,
+states of another rule, arrays that overlap."""
+import pytest
+import torch
+
+from fused_optim import FusedAdamW
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+E4M3 = 2.0 ** -4        # half a step of e4m3, relative
+LEAST = 2.0 ** -10      # half of its least subnormal
+
+
+# ---- moments in 8 bits, given as floats ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("least", [1e-45, 1e-39, 1e-37, 1.3e-36, 1e-34, 2.0 ** -110, 1e-30])
+def test_tiny_first_moments_are_held_near_zero(least):
+    """Blocks whose largest moment is below 2^-110 are held as zeros; from there on e4m3's rounding holds: half a step of the value, or of the block's largest / 448."""
+    p = torch.nn.Parameter(torch.zeros(600))
+    m = torch.zeros(600)
+    m[:10] = least * torch.linspace(-1.0, 1.0, 10)
+    m[300:310] = 0.5                                    # another block, which has to stay
+    opt = FusedAdamW([p], state_bits=8)
+    opt.set_moments(p, m, torch.zeros(600), step=3)
+    got, v = opt.moments(p)
+    assert bool((v == 0).all())
+    assert bool(((got[256:] - m[256:]).abs() <= E4M3 * m[256:].abs()).all())
+    if least < 2.0 ** -110:
+        assert bool((got[:256] == 0).all())
+    else:
+        off = (got[:256].double() - m[:256].double()).abs()
+        assert bool((off <= (E4M3 + 2.0 ** -22) * m[:256].abs().double() + 1.001 * LEAST * least / 448).all()) and bool((got[:10] != 0).any())
+
+
+def test_tiny_second_moments_are_not_lost():
+    p = torch.nn.Parameter(torch.zeros(300))
+    v = torch.full((300,), 1e-45)                       # float32's least: its root is 3.7e-23
+    opt = FusedAdamW([p], state_bits=8)
+    opt.set_moments(p, torch.zeros(300), v)
+    root = opt.moments(p)[1].double()                   # (squares of 3.7e-23 in float32: the least number or 0)
+    codes = opt.state[p]["exp_avg_rms"].float()
+    assert bool((codes > 0).all()) and bool(torch.isfinite(root).all())
