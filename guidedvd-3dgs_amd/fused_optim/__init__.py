@@ -197,10 +197,11 @@ class FusedAdamW(torch.optim.Optimizer):
                 ordered = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(x)
                 row[:p.numel()] = _in_order(ordered)
                 row = row.view(-1, BLOCK)
-                big = row.abs().amax(1)
+                finite = row.isfinite()                   # (what is not is held as e4m3's NaN and leaves its block as it is, as in the kernel)
+                big = torch.where(finite, row.abs(), 0.0).amax(1)
                 big = torch.where(big < TINY, 0.0, big)
                 scales.copy_(big / 448.0)
-                q = torch.where(big[:, None] > 0, row * (448.0 / big[:, None]), 0.0)
+                q = torch.where(big[:, None] > 0, row * (448.0 / big[:, None]), 0.0).masked_fill(~finite, float("nan"))
                 if codes is st["exp_avg_rms"]:
                     q = torch.where(row > 0, q.clamp(min=2.0 ** -9), q)      # a root above 0 is never held as 0
                 _in_order(codes.view(torch.uint8)).copy_(q.to(torch.float8_e4m3fn).view(torch.uint8).view(-1)[:p.numel()])

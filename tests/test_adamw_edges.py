@@ -39,3 +39,21 @@ def test_tiny_second_moments_are_not_lost():
     root = opt.moments(p)[1].double()                   # (squares of 3.7e-23 in float32: the least number or 0)
     codes = opt.state[p]["exp_avg_rms"].float()
     assert bool((codes > 0).all()) and bool(torch.isfinite(root).all())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_moments_that_are_not_finite_stay_with_their_element(value, device):
+    gen = torch.Generator().manual_seed(0)
+    p = torch.nn.Parameter(torch.zeros(700, device=device))
+    m, v = torch.randn(700, generator=gen).to(device), torch.rand(700, generator=gen).to(device) + 0.1
+    m[5] = m[300] = v[6] = v[301] = value
+    m[600:], m[650] = 0.0, value                        # a block with nothing else in it
+    m[512:600] = 0.0
+    opt = FusedAdamW([p], state_bits=8)
+    opt.set_moments(p, m, v)
+    for got, x in zip(opt.moments(p), (m, v)):
+        bad = ~torch.isfinite(x)
+        assert torch.equal(torch.isfinite(got), ~bad)
+        size = x[~bad].abs().max()
+        assert bool(((got - x)[~bad].abs() <= 2.2 * E4M3 * x[~bad].abs() + size * LEAST / 448).all())     # (a square: twice the root's half step, and its own square)
