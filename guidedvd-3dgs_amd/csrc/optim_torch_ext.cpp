@@ -41,7 +41,14 @@ void init(const std::string& path)
 
 void check(int rc) { TORCH_CHECK(rc == 0, "gvd_optim error ", rc, ": ", g_api.last_error()); }
 
-bool same_order(const at::Tensor& a, const at::Tensor& b) { return a.numel() <= 1 || a.strides() == b.strides(); }
+// Whether two tensors of one shape lie in the same memory order.  The stride of a dimension of size 1 moves nothing, and there are several spellings of it.
+bool same_order(const at::Tensor& a, const at::Tensor& b)
+{
+    if (a.numel() <= 1) return true;
+    for (int64_t d = 0; d < a.dim(); d++)
+        if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
 
 // A state tensor of parameter p: its type, shape, device and memory order.
 void check_state(const at::Tensor& p, const at::Tensor& t, at::ScalarType type, const char* name, int64_t bits)

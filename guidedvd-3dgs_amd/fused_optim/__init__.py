@@ -66,6 +66,11 @@ def _like(t, dtype):
     return torch.zeros_like(t, dtype=torch.uint8, memory_format=torch.preserve_format).view(dtype)
 
 
+def _same_order(a, b):
+    """Whether two tensors of one shape lie in the same memory order: the strides of dimensions of size 1 do not count."""
+    return a.numel() <= 1 or all(x == y for n, x, y in zip(a.shape, a.stride(), b.stride()) if n != 1)
+
+
 def _in_order(t):
     """t's elements as one row, in the order of memory (a view)."""
     return t.as_strided((t.numel(),), (1,))
@@ -142,7 +147,7 @@ class FusedAdamW(torch.optim.Optimizer):
         dtype = torch.float32 if bits == 32 else torch.float8_e4m3fn
         for n in names:
             t = st.get(n)
-            if t is None or t.dtype != dtype or t.shape != p.shape or t.device != p.device or t.stride() != p.stride() and p.numel() > 1:
+            if t is None or t.dtype != dtype or t.shape != p.shape or t.device != p.device or not _same_order(t, p):
                 raise RuntimeError(f"FusedAdamW: the state {n!r} does not fit its parameter {tuple(p.shape)} (state_bits={bits}): it takes {dtype} in the "
                                    f"parameter's shape, device and memory order; got "
                                    f"{None if t is None else (t.dtype, tuple(t.shape), t.stride(), str(t.device))}")
@@ -226,7 +231,7 @@ class FusedAdamW(torch.optim.Optimizer):
             for k, v in src.items():
                 if torch.is_tensor(v) and k != "step":
                     st[k] = v.detach().to(device=p.device, copy=True)
-                    if v.dtype == torch.float32 and v.shape == p.shape and st[k].stride() != p.stride():
+                    if v.dtype == torch.float32 and v.shape == p.shape and not _same_order(st[k], p):
                         st[k] = _like(p, torch.float32).copy_(v)
             step = torch.as_tensor(src["step"], dtype=torch.float32).detach()
             st["step"] = step.to(device=p.device if g["capturable"] else "cpu", copy=True).reshape(())

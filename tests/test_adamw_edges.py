@@ -57,3 +57,59 @@ def test_moments_that_are_not_finite_stay_with_their_element(value, device):
         assert torch.equal(torch.isfinite(got), ~bad)
         size = x[~bad].abs().max()
         assert bool(((got - x)[~bad].abs() <= 2.2 * E4M3 * x[~bad].abs() + size * LEAST / 448).all())     # (a square: twice the root's half step, and its own square)
+
+
+# ---- spellings of one memory order -----------------------------------------------------------------------------------------------
+def turned(n, device="cpu"):
+    """[n, 1, 3] with strides (3, 1, 1): the same memory as a fresh tensor's (3, 3, 1)."""
+    x = torch.randn(n, 3, 1, generator=torch.Generator().manual_seed(1)).to(device).transpose(1, 2).contiguous()
+    assert x.stride() == (3, 1, 1) and torch.empty_like(x, memory_format=torch.contiguous_format).stride() != x.stride()
+    return x
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dicts_go_between_spellings_of_one_order(bits):
+    p, q = torch.nn.Parameter(turned(100)), torch.nn.Parameter(turned(100).clone(memory_format=torch.contiguous_format))
+    a, b = FusedAdamW([p], state_bits=bits), FusedAdamW([q], state_bits=bits)
+    m, v = torch.randn(100, 1, 3), torch.rand(100, 1, 3)
+    for x, y, r, s in ((a, b, p, q), (b, a, q, p)):
+        x.set_moments(r, m, v, 3)
+        y.load_state_dict(x.state_dict())
+        assert all(torch.equal(i, j) for i, j in zip(x.moments(r), y.moments(s)))
+        m, v = m + 1, v + 1
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_and_gradients_of_another_spelling_are_taken_as_they_are(bits):
+    """A state set by hand has a fresh tensor's strides, and so has a gradient: both are the parameter's order, nothing is copied."""
+    fresh = lambda x: x.clone(memory_format=torch.contiguous_format)  # noqa: E731
+    p, q = torch.nn.Parameter(turned(1000, DEV)), torch.nn.Parameter(fresh(turned(1000, DEV)))
+    g = torch.randn(1000, 1, 3, device=DEV, generator=torch.Generator(device=DEV).manual_seed(0))
+    a, b = FusedAdamW([p], lr=1e-2, state_bits=bits), FusedAdamW([q], lr=1e-2, state_bits=bits)
+    for step in range(3):
+        p.grad, q.grad = g * (step + 1), g * (step + 1)
+        assert p.grad.stride() != p.stride()
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        if step:
+            a.step()
+            assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+        else:
+            a.step()
+        b.step()
+        assert torch.equal(p, q) and all(torch.equal(x, y) for x, y in zip(a.moments(p), b.moments(q)))
+        if bits == 32:
+            a.state[p].update({k: fresh(a.state[p][k]) for k in ("exp_avg", "exp_avg_sq")})
+            assert a.state[p]["exp_avg"].stride() != p.stride()
+
+
+@gpu
+def test_another_order_is_still_another_order():
+    p = torch.nn.Parameter(torch.zeros(4, 1, 3, device=DEV))
+    p.grad = torch.arange(12.0, device=DEV).view(3, 1, 4).permute(2, 1, 0)
+    opt = FusedAdamW([p], lr=1.0, weight_decay=0.0)
+    opt.step()
+    assert torch.equal(opt.state[p]["exp_avg"], 0.1 * p.grad) or bool(((opt.state[p]["exp_avg"] - 0.1 * p.grad).abs() <= 4 * 2.0 ** -24 * p.grad).all())
+    opt.state[p]["exp_avg"] = torch.zeros(3, 1, 4, device=DEV).permute(2, 1, 0)
+    with pytest.raises(RuntimeError, match="does not fit"):
+        opt.step()
