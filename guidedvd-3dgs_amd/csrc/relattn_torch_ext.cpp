@@ -16,6 +16,8 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
+#include <unordered_set>
+
 #include "../../include/gvd_relattn.h"
 
 namespace {
@@ -161,19 +163,44 @@ struct RelativeBiasAttentionBackward : torch::autograd::Node {
     }
 };
 
-// A leaf's accumulating node belongs to the stream that it was made on and lives as long as some graph of the leaf does.  A backward pass that is captured while an
-// eager graph of the same leaf lives would make that stream wait for a captured one, in the engine's thread, where the error ends the process: refused here, before.
-void refuse_foreign_accumulators(std::initializer_list<const at::Tensor*> inputs, const at::Device& device)
+// Whether a stream other than the current one takes part in a capture (it was joined to it before).  The default stream never does.
+bool captured(const c10::Stream& s)
+{
+    if (s.id() == 0) return false;
+    const c10::hip::HIPStream stream(c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s.device_index()), s.id()));
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(stream.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+
+// A node of the graph belongs to the stream that it was made on, and a leaf's accumulating node lives as long as some graph of the leaf does.  A backward pass that is
+// captured while an eager graph of the same leaf lives would make that stream wait for a captured one, in the engine's thread, where the error ends the process: refused
+// here, before.  The leaf may lie behind other nodes (a projection, a cast, a view, or the copies and views that this file makes of its arguments), so all that the
+// inputs come from are looked at: in a capture only, where a call is made once.
+void refuse_foreign_nodes(std::initializer_list<const at::Tensor*> inputs, const at::Device& device)
 {
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     TORCH_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()).stream(), &capture) == hipSuccess, "relative_bias_attention: the stream cannot be asked whether it is capturing");
     if (capture == hipStreamCaptureStatusNone) return;
     const c10::Stream now = c10::impl::VirtualGuardImpl(device.type()).getStream(device);
+    auto look_at = [&](torch::autograd::Node* node) {
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || *stream == now || captured(*stream),
+                    "relative_bias_attention: a training pass cannot be captured while an eager graph of the same leaf lives (drop its outputs first), nor on from an eager graph");
+    };
+    std::vector<torch::autograd::Node*> open;
+    std::unordered_set<torch::autograd::Node*> met;
     for (const at::Tensor* t : inputs) {
-        if (!t->requires_grad() || !t->is_leaf()) continue;
-        const auto accumulate = torch::autograd::impl::try_get_grad_accumulator(*t);
-        TORCH_CHECK(!accumulate || !accumulate->stream() || *accumulate->stream() == now,
-                    "relative_bias_attention: a training pass cannot be captured while an eager graph of the same leaf lives (drop its outputs first)");
+        if (!t->requires_grad()) continue;
+        if (!t->is_leaf()) open.push_back(t->grad_fn().get());
+        else if (const auto accumulate = torch::autograd::impl::try_get_grad_accumulator(*t)) look_at(accumulate.get());
+    }
+    while (!open.empty()) {
+        torch::autograd::Node* node = open.back();
+        open.pop_back();
+        if (!met.insert(node).second) continue;
+        look_at(node);
+        for (const torch::autograd::Edge& e : node->next_edges())
+            if (e.function) open.push_back(e.function.get());
     }
 }
 
@@ -243,7 +270,7 @@ c10::optional<at::Tensor> attend(const at::Tensor& q, at::Tensor k, at::Tensor v
             k = k.expand(shape);
             v = v.expand(shape);
         }
-        refuse_foreign_accumulators({&q, &k, &v, &table}, q.device());
+        refuse_foreign_nodes({&q, &k, &v, &table}, q.device());
         return differentiable(q, k, v, table, c);
     }
     return forward_(q, k, v, table, q_starts, c, nullptr);

@@ -151,3 +151,88 @@ def test_a_tangent_is_refused_whether_or_not_anything_needs_a_gradient(which, n)
         with torch.inference_mode():      # tangents are not propagated here, by any operator
             out = ops.relative_bias_attention(*args, 2)
     assert torch.equal(out, ops.relative_bias_attention(q, k, v, t, 2))
+
+
+# ---- captures beside eager graphs -------------------------------------------------------------------------------------------------
+def leaves_behind(which, n, H=2):
+    """Inputs that reach a leaf through other nodes: () -> (q, k, v, table) made anew from the same leaves, and the leaf."""
+    q, k, v, t, _ = inputs(2, H, n, n, torch.bfloat16, seed=n)
+    if which == "a table of another memory order":       # (a copy is made of it)
+        leaf = t.t().contiguous().t().requires_grad_(True)
+        assert not leaf.is_contiguous()
+        return lambda: (q, k, v, leaf), leaf
+    if which == "keys shared by the batch":              # (expanded)
+        leaf = k[:1].clone().requires_grad_(True)
+        return lambda: (q, leaf, v[:1], t), leaf
+    if which == "a table behind a cast":
+        leaf = t.requires_grad_(True)
+        return lambda: (q, k, v, leaf.bfloat16()), leaf
+    leaf = torch.ones(H * D, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    return lambda: (torch.relu(q * leaf) + q, k, v, t), leaf        # queries behind three nodes
+
+
+WAYS = ["a table of another memory order", "keys shared by the batch", "a table behind a cast", "queries behind three nodes"]
+
+
+@gpu
+@pytest.mark.parametrize("n", [25, 70])
+@pytest.mark.parametrize("which", WAYS)
+def test_a_capture_is_refused_where_a_leaf_behind_other_nodes_has_an_eager_graph(which, n):
+    make, leaf = leaves_behind(which, n)
+    eager = ops.relative_bias_attention(*make(), 2)                 # lives on
+    trained = eager.detach().clone()                                # (summed from unrounded weights, inference from rounded ones: other last bits)
+    with torch.no_grad():
+        inferred = ops.relative_bias_attention(*make(), 2)
+    side, graph, x = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph, stream=side):
+        x += 1
+        with pytest.raises(RuntimeError, match="eager graph"):
+            ops.relative_bias_attention(*make(), 2)
+        with torch.no_grad():
+            y = ops.relative_bias_attention(*make(), 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, inferred) and float(x[0]) == 1
+    del eager
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second, stream=side):                     # nothing lives: taken
+        out = ops.relative_bias_attention(*make(), 2)
+    for _ in range(3):
+        out.detach().zero_()
+        second.replay()
+        torch.cuda.synchronize()
+        assert out.requires_grad and torch.equal(out.detach(), trained)
+
+
+@gpu
+def test_a_capture_does_not_go_on_from_an_eager_graph():
+    q, k, v, t, _ = inputs(2, 2, 25, 25)
+    q = q.requires_grad_(True) * 1.0                                # made before the capture, on another stream
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="eager graph"):
+            ops.relative_bias_attention(q, k, v, t, 2)
+        y = ops.relative_bias_attention(q.detach(), k, v, t, 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ops.relative_bias_attention(q.detach(), k, v, t, 2))
+
+
+@gpu
+def test_two_streams_of_one_capture_share_a_leaf():
+    """The second call meets the table's accumulating node on the other stream, which is captured as well."""
+    q, k, v, t, _ = inputs(2, 2, 70, 70, torch.bfloat16)
+    t.requires_grad_(True)
+    one, two, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=one):
+        a = ops.relative_bias_attention(q, k, v, t, 2)
+        two.wait_stream(one)
+        with torch.cuda.stream(two):
+            b = ops.relative_bias_attention(q, k, v, t, 2, causal=True)
+        one.wait_stream(two)
+    for rep in range(3):
+        q.copy_(torch.randn(q.shape, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ops.relative_bias_attention(q, k, v, t, 2)) and torch.equal(b, ops.relative_bias_attention(q, k, v, t, 2, causal=True)), rep
