@@ -41,7 +41,7 @@ int fail(int code, const char* what, hipError_t e = hipSuccess)
 constexpr int MAX_TENSORS = 52;   // 52 * 76 bytes and the other arguments: below 4 KiB of kernel arguments
 constexpr int CHUNK = 2048;       // elements a workgroup: eight blocks of 8-bit moments, two rounds of 256 lanes x 4 (11.8M elements with 8-bit moments, ordinary accesses: 37.1 us; 1024 37.5, 4096 42.6)
 constexpr int BLOCK = GVD_ADAMW_BLOCK;
-constexpr long long MOST_WORKGROUPS = 1LL << 23;   // of a launch: 2^31 lanes (and 2^34 elements a tensor)
+constexpr long long MOST_WORKGROUPS = GVD_ADAMW_MOST / CHUNK;   // of a launch: 2^23, 2^31 lanes
 
 struct Table {
     gvd_adamw_tensor t[MAX_TENSORS];
@@ -363,7 +363,7 @@ int gvd_adamw_step(const gvd_adamw_tensor* tensors, int count, int param_type, i
     if (bad_betas(beta1, beta2) || !(eps >= 0.0)) return fail(-1, "gvd_adamw_step: betas must be in [0, 1) and eps at least 0");
     for (int i = 0; i < count; i++) {
         const gvd_adamw_tensor& t = tensors[i];
-        if (t.n < 0 || t.n > MOST_WORKGROUPS * CHUNK) return fail(-1, "gvd_adamw_step: a tensor's size is out of range");
+        if (t.n < 0 || t.n > GVD_ADAMW_MOST) return fail(-1, "gvd_adamw_step: a tensor's size is out of range");
         if (t.n && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale))))
             return fail(-1, "gvd_adamw_step: a tensor has a null pointer");
     }

@@ -92,6 +92,10 @@ struct Launch {
     {
         const size_t n = place.size(), k = per();
         TORCH_CHECK_TYPE(param_type() >= 0, "FusedAdamW: parameters are float32, float16 or bfloat16, not ", type);
+        // (groups are dicts that a program may change between steps)
+        TORCH_CHECK_VALUE(bits == 8 || bits == 32, "FusedAdamW: state_bits must be 8 or 32, not ", bits);
+        TORCH_CHECK_VALUE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "FusedAdamW: invalid betas (", beta1, ", ", beta2, ")");
+        TORCH_CHECK_VALUE(eps >= 0.0 && std::isfinite(eps), "FusedAdamW: invalid eps ", eps);
         const at::ScalarType moment = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
         if (!capturable) {
             hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -126,7 +130,12 @@ struct Launch {
             t.exp_avg = m.data_ptr();
             t.exp_avg_sq = v.data_ptr();
             t.n = p.numel();
-            if (lr_at[i].defined()) TORCH_CHECK(lr_at[i].device() == device, "FusedAdamW: lr is on another device than its parameters");
+            TORCH_CHECK_VALUE(t.n <= GVD_ADAMW_MOST, "FusedAdamW: a parameter of ", t.n, " elements (at most ", GVD_ADAMW_MOST, ")");
+            if (lr_at[i].defined()) {
+                TORCH_CHECK(lr_at[i].device() == device, "FusedAdamW: lr is on another device than its parameters");
+                TORCH_CHECK_VALUE(lr_at[i].scalar_type() == at::kFloat && lr_at[i].numel() == 1, "FusedAdamW: a tensor lr is one float32 on the parameters' device, not ",
+                                  lr_at[i].scalar_type(), " ", lr_at[i].sizes());
+            }
         }
         std::sort(spans.begin(), spans.end());
         for (size_t i = 1; i < n; i++)

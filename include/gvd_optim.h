@@ -13,6 +13,8 @@ extern "C" {
 
 /* Elements that share one scale where moments are held in 8 bits. */
 #define GVD_ADAMW_BLOCK 256
+/* Elements of a tensor at most. */
+#define GVD_ADAMW_MOST (1LL << 34)
 
 /* One tensor of a step.  All arrays hold n elements in the same memory order, dense; no two arrays of one call overlap.
  * state_bits 32: exp_avg, exp_avg_sq are float[n]; the scale pointers are not read.

@@ -113,3 +113,26 @@ def test_another_order_is_still_another_order():
     opt.state[p]["exp_avg"] = torch.zeros(3, 1, 4, device=DEV).permute(2, 1, 0)
     with pytest.raises(RuntimeError, match="does not fit"):
         opt.step()
+
+
+# ---- groups that change between steps ------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("change,error", [(lambda g: g.update(lr=torch.tensor(1e-3, device=DEV, dtype=torch.float64)), ValueError), (lambda g: g.update(lr=torch.zeros(2, device=DEV)), ValueError),
+                                          (lambda g: g.update(lr=torch.zeros(0, device=DEV)), ValueError), (lambda g: g.update(lr=torch.tensor(1e-3)), RuntimeError),
+                                          (lambda g: g.update(betas=(0.9, 1.0)), ValueError), (lambda g: g.update(betas=(-0.1, 0.9)), ValueError),
+                                          (lambda g: g.update(betas=(float("nan"), 0.9)), ValueError), (lambda g: g.update(eps=-1.0), ValueError),
+                                          (lambda g: g.update(eps=float("nan")), ValueError), (lambda g: g.update(state_bits=16), ValueError)])
+def test_a_group_that_cannot_be_taken_is_refused_before_another_is_stepped(change, error):
+    a, b = (torch.nn.Parameter(torch.ones(70, device=DEV)) for _ in range(2))
+    opt = FusedAdamW([dict(params=[a]), dict(params=[b], lr=torch.tensor(1e-3, device=DEV), capturable=True)])
+    for p in (a, b):
+        p.grad = torch.ones_like(p)
+    opt.step()
+    kept, old = [p.detach().clone() for p in (a, b)], dict(opt.param_groups[1])
+    change(opt.param_groups[1])
+    with pytest.raises(error):
+        opt.step()
+    assert torch.equal(a, kept[0]) and torch.equal(b, kept[1]) and float(opt.state[a]["step"]) == 1 == float(opt.state[b]["step"])
+    opt.param_groups[1].update(old)
+    opt.step()
+    assert not torch.equal(a, kept[0]) and not torch.equal(b, kept[1])
