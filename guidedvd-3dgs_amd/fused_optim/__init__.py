@@ -213,7 +213,15 @@ class FusedAdamW(torch.optim.Optimizer):
         self.state[p] = st
 
     def load_state_dict(self, state_dict):
-        """Like torch's, but the state keeps the types it was saved with (torch casts it to the parameter's)."""
+        """Like torch's, but the state keeps the types it was saved with (torch casts it to the parameter's).  A refused one leaves the optimizer as it was."""
+        before = self.state, self.param_groups           # (torch puts others in their place)
+        try:
+            self._load_state_dict(state_dict)
+        except Exception:
+            self.state, self.param_groups = before
+            raise
+
+    def _load_state_dict(self, state_dict):
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         super().load_state_dict(state_dict)
         for g in self.param_groups:

@@ -136,3 +136,26 @@ def test_a_group_that_cannot_be_taken_is_refused_before_another_is_stepped(chang
     opt.param_groups[1].update(old)
     opt.step()
     assert not torch.equal(a, kept[0]) and not torch.equal(b, kept[1])
+
+
+# ---- states of another rule or form -----------------------------------------------------------------------------------------------------
+def test_a_refused_state_leaves_the_optimizer_as_it_was():
+    p = torch.nn.Parameter(torch.randn(5, 3))
+    opt = FusedAdamW([p], lr=3e-3, weight_decay=0.0)
+    m, v = torch.randn(5, 3), torch.rand(5, 3)
+    opt.set_moments(p, m, v, 7)
+    p.grad = torch.randn(5, 3)
+    others = [torch.optim.Adam([p], lr=1.0, amsgrad=True), torch.optim.Adam([p], lr=1.0, maximize=True), torch.optim.Adam([p], lr=1.0, weight_decay=0.1)]
+    for o in others:
+        o.step()
+    dicts = [o.state_dict() for o in others]
+    short = FusedAdamW([p], lr=1.0, state_bits=8)
+    short.set_moments(p, m, v, 9)
+    dicts.append(short.state_dict())
+    dicts[-1]["param_groups"][0]["state_bits"] = 32         # its moments do not fit that
+    state, groups = opt.state, opt.param_groups
+    for d in dicts:
+        with pytest.raises((ValueError, RuntimeError)):
+            opt.load_state_dict(d)
+        assert opt.state is state and opt.param_groups is groups and opt.param_groups[0]["lr"] == 3e-3 and set(opt.state[p]) == {"step", "exp_avg", "exp_avg_sq"}
+        assert float(opt.state[p]["step"]) == 7 and torch.equal(opt.state[p]["exp_avg"], m) and torch.equal(opt.state[p]["exp_avg_sq"], v)
