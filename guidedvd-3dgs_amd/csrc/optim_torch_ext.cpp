@@ -65,6 +65,9 @@ void check_scale(const at::Tensor& p, const at::Tensor& t, const char* name)
                 "FusedAdamW: the state '", name, "' does not fit its parameter ", p.sizes());
 }
 
+typedef std::pair<const char*, const char*> Span;   // bytes that a dense tensor fills, the end excluded
+Span span(const at::Tensor& t) { return {(const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes()}; }
+
 // The tensors that go into one launch: all of one type and device, under one rule.
 struct Launch {
     at::Device device = at::kCPU;
@@ -104,7 +107,8 @@ struct Launch {
         }
         table.resize(n);
         grads.resize(n);
-        std::vector<std::pair<const char*, const char*>> spans(n);
+        std::vector<Span> written;
+        written.reserve(n * (k - 2));
         for (size_t i = 0; i < n; i++) {
             const at::Tensor &p = flat[i * k], &g = flat[i * k + 1], &step = flat[i * k + 2], &m = flat[i * k + 3], &v = flat[i * k + 4];
             TORCH_CHECK(g.layout() == at::kStrided, "FusedAdamW: sparse gradients are not supported");
@@ -123,7 +127,8 @@ struct Launch {
                 t.exp_avg_scale = flat[i * k + 5].data_ptr<float>();
                 t.exp_avg_sq_scale = flat[i * k + 6].data_ptr<float>();
             }
-            spans[i] = {(const char*)p.data_ptr(), (const char*)p.data_ptr() + p.nbytes()};
+            written.push_back(span(p));
+            for (size_t j = 3; j < k; j++) written.push_back(span(flat[i * k + j]));
             grads[i] = same_order(p, g) ? g : at::empty_like(p).copy_(g);
             t.param = p.data_ptr();
             t.grad = grads[i].data_ptr();
@@ -137,9 +142,17 @@ struct Launch {
                                   lr_at[i].scalar_type(), " ", lr_at[i].sizes());
             }
         }
-        std::sort(spans.begin(), spans.end());
-        for (size_t i = 1; i < n; i++)
-            TORCH_CHECK(spans[i].first >= spans[i - 1].second || spans[i - 1].first == spans[i - 1].second, "FusedAdamW: two parameters share memory");
+        // What the launch writes is read by no other tensor's workgroups, which run in any order.
+        written.erase(std::remove_if(written.begin(), written.end(), [](const Span& x) { return x.first == x.second; }), written.end());
+        std::sort(written.begin(), written.end());
+        for (size_t i = 1; i < written.size(); i++)
+            TORCH_CHECK(written[i].first >= written[i - 1].second, "FusedAdamW: two parameters share memory, or their states do");
+        for (size_t i = 0; i < n; i++) {
+            const Span g = span(grads[i]);
+            if (g.first == g.second || g == span(flat[i * k])) continue;   // (a gradient that is the parameter itself: each element is read before it is written)
+            const auto next = std::lower_bound(written.begin(), written.end(), Span(g.second, nullptr));   // the first that begins at or behind the gradient's end
+            TORCH_CHECK(next == written.begin() || std::prev(next)->second <= g.first, "FusedAdamW: a gradient shares memory with a parameter or a state that the step writes");
+        }
     }
 
     void run()

@@ -159,3 +159,71 @@ def test_a_refused_state_leaves_the_optimizer_as_it_was():
             opt.load_state_dict(d)
         assert opt.state is state and opt.param_groups is groups and opt.param_groups[0]["lr"] == 3e-3 and set(opt.state[p]) == {"step", "exp_avg", "exp_avg_sq"}
         assert float(opt.state[p]["step"]) == 7 and torch.equal(opt.state[p]["exp_avg"], m) and torch.equal(opt.state[p]["exp_avg_sq"], v)
+
+
+# ---- arrays that overlap ---------------------------------------------------------------------------------------------------------------
+def stepped(bits=32, count=3, n=300):
+    base = torch.ones(count * n, device=DEV)
+    params = [torch.nn.Parameter(base[i * n:(i + 1) * n]) for i in range(count)]       # side by side in one piece of memory
+    opt = FusedAdamW(params, lr=1e-2, state_bits=bits)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    return opt, params, base
+
+
+def refused(opt, params, word):
+    kept, steps = [p.detach().clone() for p in params], [float(opt.state[p]["step"]) for p in params]
+    with pytest.raises(RuntimeError, match=word):
+        opt.step()
+    assert all(torch.equal(p, x) for p, x in zip(params, kept)) and steps == [float(opt.state[p]["step"]) for p in params]
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_that_share_memory_are_refused(bits):
+    for name in ("exp_avg", "exp_avg_sq") if bits == 32 else ("exp_avg", "exp_avg_rms", "exp_avg_scale", "exp_avg_rms_scale"):
+        opt, params, _ = stepped(bits)
+        opt.state[params[2]][name] = opt.state[params[0]][name]
+        refused(opt, params, "share")
+    if bits == 32:
+        opt, params, base = stepped()
+        opt.state[params[1]]["exp_avg_sq"] = opt.state[params[1]]["exp_avg"]           # of one parameter
+        refused(opt, params, "share")
+        opt, params, base = stepped()
+        opt.state[params[1]]["exp_avg"] = base[:300]                                   # with a parameter
+        refused(opt, params, "share")
+        opt, params, base = stepped()
+        both = torch.zeros(400, device=DEV)
+        opt.state[params[0]]["exp_avg"], opt.state[params[2]]["exp_avg"] = both[:300], both[100:]      # in part
+        refused(opt, params, "share")
+
+
+@gpu
+@pytest.mark.parametrize("begin", [0, 1, 150, 299, 450, 600])
+def test_a_gradient_that_the_step_would_write_is_refused(begin):
+    """Three parameters side by side and a gradient over them that belongs to the second: only its own place exactly is taken."""
+    opt, params, base = stepped()
+    params[1].grad = base[begin:begin + 300]
+    refused(opt, params, "gradient shares memory")
+    params[1].grad = opt.state[params[0]]["exp_avg"]
+    refused(opt, params, "gradient shares memory")
+
+
+@gpu
+def test_gradients_that_nothing_writes_are_taken():
+    opt, params, base = stepped()
+    others = [torch.nn.Parameter(torch.ones(300, device=DEV)) for _ in params]
+    ref = FusedAdamW(others, lr=1e-2)
+    one = torch.linspace(-1, 1, 300, device=DEV)
+    for p in others:
+        p.grad = torch.ones_like(p)
+    ref.step()
+    for p in (*params, *others):
+        p.grad = one                                                                   # the same for all
+    opt.step()
+    ref.step()
+    params[1].grad, others[1].grad = params[1].detach(), others[1].detach().clone()    # the parameter itself, in its own place
+    opt.step()
+    ref.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, others))
