@@ -16,6 +16,8 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
+#include <algorithm>
+#include <climits>
 #include <unordered_set>
 
 #include "../../include/gvd_relattn.h"
@@ -81,10 +83,11 @@ std::pair<long long, long long> strides(const at::Tensor& t, const Config& c)
 gvd_relattn_problem problem(const at::Tensor& q, const at::Tensor& k, const at::Tensor& out, const at::Tensor& table, const at::Tensor& q_starts, const Config& c)
 {
     gvd_relattn_problem p = {};
-    p.B = (int)q.size(c.batch_dim());
-    p.H = (int)c.heads;
-    p.Nq = (int)q.size(c.row_dim());
-    p.Nk = (int)k.size(c.row_dim());
+    auto whole = [](int64_t n) { return (int)std::min<int64_t>(n, INT_MAX); };   // (an expanded tensor may have any size: what an int does not hold is refused as too large)
+    p.B = whole(q.size(c.batch_dim()));
+    p.H = whole(c.heads);
+    p.Nq = whole(q.size(c.row_dim()));
+    p.Nk = whole(k.size(c.row_dim()));
     p.D = (int)(q.size(2) / c.heads);
     p.is_bf16 = q.scalar_type() == at::kBFloat16;
     p.table_type = table.scalar_type() == at::kFloat ? 0 : table.scalar_type() == at::kHalf ? 1 : 2;

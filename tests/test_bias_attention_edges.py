@@ -236,3 +236,13 @@ def test_two_streams_of_one_capture_share_a_leaf():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, ops.relative_bias_attention(q, k, v, t, 2)) and torch.equal(b, ops.relative_bias_attention(q, k, v, t, 2, causal=True)), rep
+
+
+# ---- sizes beyond 32 bits ------------------------------------------------------------------------------------------------------------
+@gpu
+def test_sizes_that_an_int_does_not_hold_are_refused():
+    """Expanded tensors take no memory: 2^32 + 5 keys would be 5 in 32 bits."""
+    q, k, v, t, _ = inputs(1, 1, 3, 1)
+    for n in (2 ** 31, 2 ** 32 + 5, 2 ** 25):
+        with pytest.raises(RuntimeError, match="too many"):
+            ops.relative_bias_attention(q, k.expand(1, n, D), v.expand(1, n, D), t, 1)
