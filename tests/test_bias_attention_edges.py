@@ -3,6 +3,7 @@ device, captures beside eager graphs, scores that grow along the keys, batches o
 import pytest
 import torch
 
+import test_relative_attention as plain
 from lvdm_amd import ops, relative
 
 gpu = pytest.mark.gpu
@@ -19,8 +20,8 @@ def inputs(B, H, Nq, Nk, dtype=torch.float16, table_dtype=torch.float32, buckets
 
 def formula(q, k, v, t, H, g, d32, **kw):
     """Results in 64 bits, by the explicit form and autograd, and how far a kernel may be: d32 is the relative error of a weight before it is rounded; weights and dS are
-    rounded to the rows' type (u), results once more.  dS = P (dP - delta): each factor d32 off, delta as a sum of weights times dP, and dQ forms it from a delta that the
-    rounded output gave and takes the difference off again (2 u of a row's sum of P |dP| at most)."""
+    rounded to the rows' type (u), results once more.  dS = P (dP - delta): each factor d32 off, delta as a sum of weights times dP.  dQ forms dS from the delta that the
+    rounded output gave, e_delta off at most, and takes (that) P K off again: the roundings of both see it."""
     u, u_t = torch.finfo(q.dtype).eps / 2, torch.finfo(t.dtype).eps / 2
     small = 2.0 ** -24 if q.dtype == torch.float16 else 2.0 ** -126
     leaves = [x.detach().double().requires_grad_(True) for x in (q, k, v, t)]
@@ -41,7 +42,8 @@ def formula(q, k, v, t, H, g, d32, **kw):
     spread = (p * dp.abs()).sum(-1, keepdim=True)
     ds = p * (dp - (p * dp).sum(-1, keepdim=True))
     e_p = (u + d32) * p + small
-    e_ds = u * ds.abs() + 2 * u * u * p * spread * 4 + 3 * d32 * p * (dp.abs() + spread) + small
+    e_delta = 2 * (u + d32) * (G.abs() * (p @ V.abs())).sum(-1, keepdim=True)
+    e_ds = u * (ds.abs() + 2 * p * e_delta) + 3 * d32 * p * (dp.abs() + spread) + small
     e_t = torch.zeros_like(want["dtable"]).index_add_(0, bucket.reshape(-1), (3 * d32 * p * (dp.abs() + spread)).sum(0).permute(1, 2, 0).reshape(-1, H))
     err = dict(out=rows(e_p @ V.abs()), dq=rows(e_ds @ K.abs()) * scale, dk=rows(e_ds.transpose(-1, -2) @ Q.abs()) * scale, dv=rows(e_p.transpose(-1, -2) @ G.abs()), dtable=e_t)
     return want, {n: 1.01 * e + (u_t if n == "dtable" else u) * want[n].abs() + 2.0 ** -24 for n, e in err.items()}
@@ -246,3 +248,63 @@ def test_sizes_that_an_int_does_not_hold_are_refused():
     for n in (2 ** 31, 2 ** 32 + 5, 2 ** 25):
         with pytest.raises(RuntimeError, match="too many"):
             ops.relative_bias_attention(q, k.expand(1, n, D), v.expand(1, n, D), t, 1)
+
+
+# ---- scores that are large, or grow along the keys ---------------------------------------------------------------------------------------
+SHAPES = [(1, 2, 25, 30), (1, 2, 3, 700), (1, 2, 140, 700), (2, 3, 300, 400), (1, 2, 70, 1100), (3, 8, 600, 640)]      # every form: short, few, rows whole and in parts
+
+
+@gpu
+@pytest.mark.parametrize("B,H,nq,nk", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large_scores_and_their_gradients(B, H, nq, nk, dtype):
+    """Scores of several hundred.  64 products of sum |q k| < 128 at a scale of 4 leave a score 64 x 2^-24 x 512 = 2^-9 off at most, a weight (over their sum) 2^-8; the type's
+    roundings are no larger than elsewhere."""
+    q, k, v, t, g = inputs(B, H, nq, nk, dtype, seed=6)
+    heads = lambda x: x.double().reshape(*x.shape[:2], H, D).transpose(1, 2)  # noqa: E731
+    assert float((heads(q).abs() @ heads(k).abs().transpose(-1, -2)).max()) < 128
+    t[7] += 200.0
+    want, err = formula(q, k, v, t, H, g, 2.0 ** -8, scale=4.0)
+    close(kernels(q, k, v, t, H, g, scale=4.0), want, err)
+    with torch.no_grad():
+        close(dict(out=ops.relative_bias_attention(q, k, v, t, H, scale=4.0)), dict(out=want["out"]), err)
+
+
+@gpu
+@pytest.mark.parametrize("B,H,nq,nk", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rise", [0.5, 3.0, 10.0, -5.0])
+def test_scores_that_grow_or_fall_from_tile_to_tile(rise, dtype, B, H, nq, nk):
+    """By `rise` every 64 keys, 0.5 and 3 below what moves the running maximum (a row's sum of a tile above 2^15) for some tiles, 10 above it at once.  Sums |q k| / 8 stay below
+    17 x 10 + 16 < 192: a score is 64 x 2^-24 x 192 < 2^-10 off, a weight 2^-9."""
+    q, k, v, t, g = inputs(B, H, nq, nk, dtype, seed=7)
+    steps = (torch.arange(nk, device=DEV) // 64).float() * rise
+    for h in range(H):
+        q[:, :, h * D] = 8.0
+        k[:, :, h * D] = steps.to(dtype)
+    heads = lambda x: x.double().reshape(*x.shape[:2], H, D).transpose(1, 2)  # noqa: E731
+    assert float((heads(q).abs() @ heads(k).abs().transpose(-1, -2)).max()) / 8 < 192
+    want, err = formula(q, k, v, t, H, g, 2.0 ** -9)
+    close(kernels(q, k, v, t, H, g), want, err)
+    with torch.no_grad():
+        close(dict(out=ops.relative_bias_attention(q, k, v, t, H)), dict(out=want["out"]), err)
+
+
+# ---- many short rows ---------------------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [33, 48, 63, 64])
+def test_more_than_32_frames_of_many_pixels(n, dtype):
+    """Several workgroups a compute unit one after the other, each with a part of its rows in use."""
+    q, k, v, t, g = plain.inputs(900, 3, n, n, dtype, frame_major=True, seed=n)
+    plain.check(q, k, v, t, g, 3, frame_major=True)
+    lens = torch.arange(900, device=DEV, dtype=torch.int32) % (n + 2)
+    plain.check(q, k, v, t, g, 3, frame_major=True, causal=True, kv_lens=lens)
+
+
+@gpu
+@pytest.mark.parametrize("nq", [1, 2, 4])
+def test_new_tokens_of_many_sequences(nq):
+    q, k, v, t, _ = plain.inputs(1500, 2, nq, 70, torch.bfloat16, seed=nq)
+    lens = torch.arange(1500, device=DEV, dtype=torch.int32) % 71
+    plain.check(q, k, v, t, None, 2, train=False, causal=True, bidirectional=False, q_start=(lens - nq).to(torch.int32), kv_lens=lens)
