@@ -74,6 +74,11 @@ int make_geo(const gvd_relattn_problem* p, Geo& g, const char* who)
 
 namespace {
 
+// What a row's weights are divided by, from their sum: 0 where the row sees nothing (its sum is 0 exactly, else at least one weight is about 1), and its log-sum-exp.
+// A sum of NaN (a NaN or an infinity among the row's scores) stays one.
+__device__ __forceinline__ float over(float sum) { return sum == 0.f ? 0.f : 1.0f / sum; }
+__device__ __forceinline__ float lse_of(float max, float sum) { return sum == 0.f ? INFINITY : max + __builtin_amdgcn_logf(sum); }
+
 // ---- general rows ------------------------------------------------------------------------------------------------------------
 // The vector unit bounds this kernel: 32 exponentials a lane, query block and tile, against 16 products of the matrix unit.  9216 rows, 5 heads: 147 us, 740 TFLOP/s; 20 heads
 // 540, 805; 2304 rows, 10 heads: 31.7.  So the loop does little else:
@@ -320,8 +325,8 @@ k_rel_fwd(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
             }
             continue;
         }
-        if (LSE && hi == 0) lse[(size_t)bh * g.Nq + query[qi]] = l[qi] > 0.f ? m[qi] + __builtin_amdgcn_logf(l[qi]) : INFINITY;
-        const float inv = l[qi] > 0.f ? 1.0f / l[qi] : 0.f;   // a row that sees nothing: zeros
+        if (LSE && hi == 0) lse[(size_t)bh * g.Nq + query[qi]] = lse_of(m[qi], l[qi]);
+        const float inv = over(l[qi]);
         T* orow = out + (size_t)b * g.o_bs + (size_t)h * 64 + (size_t)query[qi] * (size_t)g.o_rs;
 #pragma unroll
         for (int rg = 0; rg < 4; rg++) {
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __re
         o.x += __shfl_xor(o.x, w, LN); o.y += __shfl_xor(o.y, w, LN);
         o.z += __shfl_xor(o.z, w, LN); o.w += __shfl_xor(o.w, w, LN);
     }
-    const float inv = total > 0.f ? 1.0f / total : 0.f;
+    const float inv = over(total);
     if (lane < 16) {
         const long long bh = row / g.Nq;
         const int n = (int)(row - bh * g.Nq), b = (int)(bh / g.H), h = (int)(bh - (long long)b * g.H);
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __re
         w.x = Tr<T>::pack2(o.x * inv, o.y * inv);
         w.y = Tr<T>::pack2(o.z * inv, o.w * inv);
         *reinterpret_cast<uint2*>(out + (size_t)b * g.o_bs + (size_t)n * g.o_rs + (size_t)h * 64 + d0) = w;
-        if (lse && lane == 0) lse[row] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+        if (lse && lane == 0) lse[row] = lse_of(top, total);
     }
 }
 
@@ -486,8 +491,8 @@ __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restr
             o1 = Tr<T>::mfma(transposed_operand(&rows[0][0], PITCH, 16 * k2, 32, lane), pf, o1);
         }
         wave_order();
-        const bool empty = !(l > 0.f) || len == 0;   // (a length of zero: row 0 of V was loaded, whatever it holds)
-        if (lse && hi == 0 && r32 < g.Nq) lse[((size_t)b * g.H + h) * g.Nq + r32] = empty ? INFINITY : mt + __builtin_amdgcn_logf(l);
+        const bool empty = l == 0.f;   // (its result is not formed as 0 times what was summed: with a length of zero row 0 of V was loaded, whatever it holds)
+        if (lse && hi == 0 && r32 < g.Nq) lse[((size_t)b * g.H + h) * g.Nq + r32] = lse_of(mt, l);
         const float inv = 1.0f / l;
 #pragma unroll
         for (int rg = 0; rg < 4; rg++) {
@@ -633,8 +638,8 @@ __global__ void __launch_bounds__(256) k_rel_few(const Geo g, const T* __restric
             part_o[row * 64 + d] = o;
             if (d == 0) part_ml[row] = make_float2(top, total);
         } else {
-            out[(size_t)b * g.o_bs + (size_t)i * g.o_rs + (size_t)h * 64 + d] = (T)(total > 0.f ? o / total : 0.f);
-            if (lse && d == 0) lse[(size_t)bh * g.Nq + i] = total > 0.f ? top + __builtin_amdgcn_logf(total) : INFINITY;
+            out[(size_t)b * g.o_bs + (size_t)i * g.o_rs + (size_t)h * 64 + d] = (T)(total == 0.f ? 0.f : o / total);
+            if (lse && d == 0) lse[(size_t)bh * g.Nq + i] = lse_of(top, total);
         }
     }
 }

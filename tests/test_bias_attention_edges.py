@@ -308,3 +308,33 @@ def test_new_tokens_of_many_sequences(nq):
     q, k, v, t, _ = plain.inputs(1500, 2, nq, 70, torch.bfloat16, seed=nq)
     lens = torch.arange(1500, device=DEV, dtype=torch.int32) % 71
     plain.check(q, k, v, t, None, 2, train=False, causal=True, bidirectional=False, q_start=(lens - nq).to(torch.int32), kv_lens=lens)
+
+
+# ---- values that are not finite -------------------------------------------------------------------------------------------------------
+ALL_FORMS = [(25, 25), (32, 7), (1, 40), (3, 40), (2, 3000), (70, 70), (40, 3000), (300, 200)]
+
+
+@gpu
+@pytest.mark.parametrize("nq,nk", ALL_FORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("what,value", [("q", float("nan")), ("q", float("inf")), ("k", float("nan")), ("k", float("-inf")), ("v", float("nan"))])
+def test_a_score_that_is_no_number_is_not_answered_with_zeros(what, value, dtype, nq, nk):
+    """The rows that are NaN by the formula are NaN, with and without gradients, and so are the gradients (a loss scaler looks there); all others are as they were."""
+    q, k, v, t, g = inputs(2, 2, nq, nk, dtype)
+    want, err = formula(q, k, v, t, 2, g, 2.0 ** -14)
+    n = min(nq, nk) - 1
+    {"q": q, "k": k, "v": v}[what][1, n] = value
+    leaves = [x.detach().double().requires_grad_(True) for x in (q, k, v, t)]
+    out = relative.relative_bias_attention_math(*leaves, 2)
+    bad = out.isnan()
+    assert bool(bad[1].all() if what != "q" else bad[1, n].all()) and not bool(bad[0].any())
+    got = kernels(q, k, v, t, 2, g)
+    with torch.no_grad():
+        plain_out = ops.relative_bias_attention(q, k, v, t, 2)
+    for x in (got["out"], plain_out):
+        assert torch.equal(x.isnan(), bad)
+        assert bool(((x.double() - want["out"]).abs() <= err["out"])[~bad].all())
+    for name, y in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, g.double())):
+        assert bool(got[name].isnan()[y.isnan()].all()), name
+    for name in ("dq", "dk", "dv"):
+        assert bool(((got[name].double() - want[name]).abs() <= err[name])[0].all()), name
