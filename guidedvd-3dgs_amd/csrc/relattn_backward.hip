@@ -119,6 +119,10 @@ k_rel_dq(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T*
         gf[ks] = *reinterpret_cast<const vec8*>(d_o + grow + 16 * ks + 8 * hi);
     }
     const float L = valid ? lse[(size_t)bh * g.Nq + query] : INFINITY;   // (infinite: every weight of the row is 0)
+    if (L == INFINITY) {   // such a row has no gradient, whatever its dO holds: a NaN times a weight of 0 would not be 0
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) gf[ks] = vec8{};
+    }
     float Dl = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
@@ -222,6 +226,7 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     __shared__ __attribute__((aligned(16))) Tiles<T> tiles;   // a: Q, b: dO
     __shared__ __attribute__((aligned(16))) float sRow[2][2][64];   // -lse and -delta of a tile's rows
     __shared__ float sFar[8][2];
+    __shared__ int sNone;   // whether some row may see nothing
     __shared__ float sSkew[8][16 * 48];
     extern __shared__ __attribute__((aligned(16))) float sBias[];   // the bias, then 8 arrays of sums by distance
     const int blen = bias_len(g.reach), span = g.reach + PAD;
@@ -271,7 +276,11 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     if (q_lo < g.Nq) prefetch(q_lo);
     for (int e = tid; e < 8 * blen; e += 512) sBias[blen + e] = 0.f;
     for (int e = lane; e < 16 * 48; e += 64) sSkew[wave][e] = 0.f;
-    fill_bias<true>(g, h, sBias, tid, 512);
+    // Rows that see nothing: those before the first key where causal, and where entries mask their buckets any row (a length of zero walks no queries).  Their weights are 0, and
+    // their dO, whatever it holds, is put to 0 in LDS, tile by tile; where there can be none of them the loop pays one scalar branch.
+    if (tid == 0) sNone = g.causal && start < 0;
+    __syncthreads();
+    if (fill_bias<true>(g, h, sBias, tid, 512)) sNone = 1;
     if (q_lo < g.Nq) {
         commit(q_lo, 0);
         prefetch(q_lo + 64);
@@ -279,10 +288,15 @@ k_rel_dkv(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T
     __syncthreads();
     const float far_ahead = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sBias[0])));
     const float far_past = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sBias[blen - 1])));
+    const bool none = __builtin_amdgcn_readfirstlane(sNone);
     // S starts from the bias; lse is subtracted behind the products, in the exponent: as a start it would be some 1 / c times larger than what is summed, and its
     // rounding steps with it (a table's gradient in 32 bits at 2304 rows: 1e-6 off, 7e-7 this way, where 32 bits throughout are 7e-7 off).
     int buf = 0;
     for (int qt = q_lo; qt < g.Nq; qt += 64, buf ^= 1) {
+        if (none) {   // (the same for the whole workgroup)
+            if (sRow[buf][0][tid >> 3] == -INFINITY) tile_commit(vec8{}, tid, tiles.b[buf]);
+            __syncthreads();
+        }
         const int first = start + qt + half;   // position of the block's first query
         const bool past = kw + 31 - first <= -g.reach, ahead = kw - first - 31 >= g.reach;
         f16v s, dp;
@@ -519,6 +533,15 @@ __global__ void __launch_bounds__(256, 2) k_rel_short_bwd(const Geo g, const T* 
         }
         load_kv(b + step < nb ? b + step : b);   // in flight under everything below
         wave_order();
+        if (__any(L == INFINITY && r32 < g.Nq)) {   // rows that see nothing have no gradient, whatever their dO (and, with a length of zero, their query) holds
+            if (L == INFINITY)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    *reinterpret_cast<vec8*>(&sG[wave][r32][32 * hi + 8 * i]) = vec8{};
+                    if (len == 0) *reinterpret_cast<vec8*>(&sQ[wave][r32][32 * hi + 8 * i]) = vec8{};
+                }
+            wave_order();
+        }
         // ---- a query per lane ----
         f16v sT, dpT = {};
 #pragma unroll

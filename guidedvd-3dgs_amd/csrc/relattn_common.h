@@ -56,11 +56,17 @@ __device__ __forceinline__ float start_value(const Geo& g, float bias)
 // Whether results do not depend on an entry: where it masks its bucket, and where another value counts in its place.
 __device__ __forceinline__ bool without_gradient(float bias) { return bias <= MASKS_AT || bias > MOST; }
 
-// MIRRORED: descending distances, for blocks whose registers run over queries.
+// MIRRORED: descending distances, for blocks whose registers run over queries.  Returns whether one of the lane's distances is masked.
 template <bool MIRRORED = false>
-__device__ __forceinline__ void fill_bias(const Geo& g, int h, float* sBias, int tid, int nt)
+__device__ __forceinline__ bool fill_bias(const Geo& g, int h, float* sBias, int tid, int nt)
 {
-    for (int e = tid; e < bias_len(g.reach); e += nt) sBias[e] = start_value(g, table_at(g, bucket_of(g, MIRRORED ? g.reach + PAD - e : e - g.reach - PAD), h));
+    bool masked = false;
+    for (int e = tid; e < bias_len(g.reach); e += nt) {
+        const float x = start_value(g, table_at(g, bucket_of(g, MIRRORED ? g.reach + PAD - e : e - g.reach - PAD), h));
+        masked |= x == -INFINITY;
+        sBias[e] = x;
+    }
+    return masked;
 }
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }

@@ -103,7 +103,7 @@ def relative_bias_attention_math(q, k, v, table, heads, *, max_distance=128, bid
     s = s.masked_fill(~seen[:, None], float("-inf"))
     empty = (s == float("-inf")).all(-1, keepdim=True)
     p = s.masked_fill(empty, 0.0).softmax(-1).masked_fill(empty, 0.0)
-    out = torch.matmul(p, vh).permute(0, 2, 1, 3).reshape(B, Nq, C).to(q.dtype)
+    out = torch.matmul(p, vh).masked_fill(empty, 0.0).permute(0, 2, 1, 3).reshape(B, Nq, C).to(q.dtype)     # (no gradient passes there, whatever it holds)
     return out.transpose(0, 1).contiguous() if frame_major else out
 
 

@@ -47,7 +47,7 @@ int gvd_relattn_fwd(const gvd_relattn_problem* p, const void* q, const void* k, 
                     void* workspace, void* stream);
 
 /* Gradients of q, k, v and the table from d_out, with `out` and `lse` of the forward.  All of dq, dk, dv, dtable are written (rows of dk, dv behind
- * len_b with zeros).  The table's gradient is summed in a fixed order. */
+ * len_b with zeros).  d_out of a query that sees nothing goes into no result.  The table's gradient is summed in a fixed order. */
 int gvd_relattn_bwd(const gvd_relattn_problem* p, const void* q, const void* k, const void* v, const void* table, const void* out, const void* d_out,
                     const float* lse, void* dq, void* dk, void* dv, void* dtable, void* workspace, void* stream);
 

@@ -338,3 +338,57 @@ def test_a_score_that_is_no_number_is_not_answered_with_zeros(what, value, dtype
         assert bool(got[name].isnan()[y.isnan()].all()), name
     for name in ("dq", "dk", "dv"):
         assert bool(((got[name].double() - want[name]).abs() <= err[name])[0].all()), name
+
+
+def nothing_seen(n, way, frame_major=False, device=DEV):
+    """(arguments, which [batch, query] see nothing) of two batch entries."""
+    none = torch.zeros(2, n, dtype=torch.bool, device=device)
+    if way == "causal":
+        none[:, :min(3, n)] = True
+        return dict(causal=True, q_start=-3), none
+    if way == "lengths":
+        none[0] = True
+        return dict(kv_lens=torch.tensor([0, n], dtype=torch.int32, device=device)), none
+    return dict(causal=True, bidirectional=False, max_distance=33), none      # ("table": the entries of the nearest distances mask, so the first rows see nothing)
+
+
+@pytest.mark.parametrize("way", ["causal", "lengths"])
+def test_the_explicit_forms_rows_that_see_nothing_have_no_gradient(way):
+    n, H = 7, 2
+    gen = torch.Generator().manual_seed(0)
+    q, k, v, g = (torch.randn(2, n, H * D, generator=gen) for _ in range(4))
+    t = torch.randn(8, H, generator=gen)
+    kw, none = nothing_seen(n, way, device="cpu")
+
+    def grads(g):
+        leaves = [x.clone().requires_grad_(True) for x in (q, k, v, t)]
+        return torch.autograd.grad(relative.relative_bias_attention_math(*leaves, H, **kw), leaves, g)
+    for value in (float("nan"), float("inf")):
+        assert all(torch.equal(x, y) for x, y in zip(grads(g.masked_fill(none[..., None], value)), grads(g.masked_fill(none[..., None], 0.0))))
+
+
+@gpu
+@pytest.mark.parametrize("n,frame_major", [(1, False), (25, True), (32, False), (70, False), (333, False)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("way", ["causal", "lengths", "table"])
+def test_rows_that_see_nothing_have_no_gradient_whatever_their_outputs_gradient_holds(way, dtype, n, frame_major):
+    H = 2
+    q, k, v, t, g = inputs(2, H, n, n, dtype, frame_major=frame_major, seed=n)
+    kw, none = nothing_seen(n, way)
+    if way == "table":
+        t[:5] = float("-inf")
+        none[:, :min(5, n)] = True
+    kw["frame_major"] = frame_major
+    rows = (none.t() if frame_major else none)[..., None]
+    want = kernels(q, k, v, t, H, g.masked_fill(rows, 0.0), **kw)
+    assert all(bool(torch.isfinite(x).all()) for x in want.values()) and bool((want["dv"] != 0).any() if n > 5 else True)
+    for value in (float("nan"), float("inf"), 1.0):
+        got = kernels(q, k, v, t, H, g.masked_fill(rows, value), **kw)
+        for name, x in want.items():
+            assert torch.equal(got[name], x), (name, value)
+    if way == "lengths":                     # queries of an empty entry are whatever was there
+        q2 = q.clone()
+        (q2[:, 0] if frame_major else q2[0]).fill_(float("nan"))
+        got = kernels(q2, k, v, t, H, g, **kw)
+        for name, x in kernels(q, k, v, t, H, g, **kw).items():
+            assert torch.equal(got[name], x), name
