@@ -13,8 +13,8 @@
 //   k_rel_table   sums the partial rows, 64 bits; an entry that masks or that counts as another value has no gradient
 // P and dS are rounded to the inputs' 16 bits as operands of the second products, the only type the matrix unit takes at this rate: 2^-8 (bf16) or 2^-11 (fp16) of each at most, which sums of
 // many terms average; the table is summed from dS in 32 bits.
-// Bound by instruction issue (two waves a SIMD, 200 registers): 2304 rows, 10 heads, 180 workgroups: 43 and 53 us; 9216 rows, 5 heads: 282 and 340 us, 770 and 640 TFLOP/s of 4
-// products each.
+// Bound by instruction issue (two waves a SIMD, 200 registers), and by the workgroups' number: 2304 rows, 10 heads, 180 workgroups on 256 CUs: 37 and 48 us in a loop of training passes, with
+// or without a causal mask (a launch lasts as long as its longest walk); 9216 rows, 5 heads: 263 and 328 us, 830 and 660 TFLOP/s of 4 products each.
 // Up to 32 queries and keys: k_rel_short_bwd, a wave an item as in the forward; the wave's head is fixed, so dS is summed over its items in registers and goes
 // into buckets once.
 #include "relattn_common.h"

@@ -80,11 +80,14 @@ __device__ __forceinline__ float over(float sum) { return sum == 0.f ? 0.f : 1.0
 __device__ __forceinline__ float lse_of(float max, float sum) { return sum == 0.f ? INFINITY : max + __builtin_amdgcn_logf(sum); }
 
 // ---- general rows ------------------------------------------------------------------------------------------------------------
-// The vector unit bounds this kernel: 32 exponentials a lane, query block and tile, against 16 products of the matrix unit.  9216 rows, 5 heads: 147 us, 740 TFLOP/s; 20 heads
-// 540, 805; 2304 rows, 10 heads: 31.7.  So the loop does little else:
+// Per query block and tile 32 exponentials a lane, with their products, roundings and sums some 770 cycles of a SIMD's vector unit, and 16 products of the matrix unit, 512 cycles.  The two take
+// turns: at 9216 rows, 5 heads about 65 us of the one and 84 of the other (at a large product's rate), 134 to 145 us in all, 750 to 810 TFLOP/s; 20 heads 507, 860; 2304 rows, 10 heads: 31.7, with LSE 27 in a
+// loop of training passes.  So the loop does little else:
 //   * the maximum is not looked for: weights are formed with the running one, and a row sum above 2^15 (always for the first tile: the maximum starts
 //     below every score) sends the block through the exact path.  Numerators and denominator share the maximum, so any one that keeps weights finite
 //     gives the exact softmax;
+//   * weights are rounded to the rows' type, the only operands that the matrix unit takes at this rate: half a step of each, 2^-11 or 2^-8, which the sum over keys averages (2.9e-4 of the
+//     output's norm in fp16, 2.3e-3 in bf16; rounding the output alone leaves 2.1e-4 and 1.7e-3);
 //   * each half wave keeps its own row sum, of the rounded weights (one dot product for two), or, where the backward will build on it (LSE), of the unrounded
 //     ones: its weights sum to 1 in 32 bits then, which the table's gradient needs; the halves meet at the end;
 //   * a block whose distances share one bias adds it to the exponent's shift, and its products start from the matrix unit's own zero.
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(256) k_rel_join(const Geo g, const float* __re
 
 // ---- up to 32 queries and keys -------------------------------------------------------------------------------------------------
 // The whole problem of an item is 3 x 32 x 128 bytes in and 32 x 128 out: memory.  A wave keeps one head (its stride over items is a multiple of H),
-// so its 16 biases a lane stay in registers over all its items; the next item's rows are requested as soon as this one's registers are free.  Rows are
+// so its 16 biases a lane stay in registers over all its items (from 33 queries or keys on there is no such form); the next item's rows are requested as soon as this one's registers are free.  Rows are
 // read whole, 8 lanes each, and take their operand forms through one piece of LDS, Q then K then V then the result (LDS operations of a wave keep their order).
 template <typename T>
 __global__ void __launch_bounds__(256) k_rel_short(const Geo g, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,

@@ -1,6 +1,6 @@
 // relattn_torch_ext.cpp -- relative_bias_attention as one node of the autograd graph over the C-ABI (include/gvd_relattn.h): checks of arguments, strides, outputs,
 // workspaces, and the backward without Python.  No kernel lives here.  With a Python autograd function a training pass took 180 us of host time, as much
-// as its kernels at the sizes of a temporal layer; here it takes 46 to 80 by the machine, of which autograd's engine takes 17 to 33 for any graph.
+// as its kernels at the sizes of a temporal layer; here it takes 42 to 80 by the machine, of which autograd's engine takes 17 to 33 for any graph.
 //
 // Plain C++ (g++); the entry points are resolved from the library path that Python hands to init(), so A/B builds share one instance.
 #include <torch/extension.h>

@@ -83,7 +83,9 @@ class FusedAdamW(torch.optim.Optimizer):
         p = (1 - lr weight_decay) p - lr / (1 - beta1^t)  m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 
     in 32 bits, rounded once to the parameter's type.  Parameters: float32, float16 or bfloat16 on a ROCm device, dense (any memory
-    order); gradients of the same type, shape and device (another memory order is copied).  Every argument may differ by parameter group.
+    order); gradients of the same type, shape and device (another memory order is copied).  Every argument may differ by parameter group.  Parameters, states
+    and gradients must not share memory (a gradient may belong to several parameters, or be its own parameter): step() refuses them.  What it refuses
+    it refuses before anything is counted or launched.
 
     state_bits   32, or 8: m and sqrt(v) as e4m3 with one float scale per 256 elements, rounded stochastically from a hash of (seed, the
                  parameter's place among all of the optimizer's, step, element) -- unbiased, and the same run gives the same result.  State:
@@ -254,8 +256,8 @@ class FusedAdamW(torch.optim.Optimizer):
         ext().step(self, self.param_groups, self.state)
         return loss
 
-    # torch.optim.Optimizer wraps the step of its classes in a profiler's range and the calls of registered hooks: 6 us where there is neither, more than all else that the
-    # host does for four small tensors (5.3 us).  So the wrapped step is called where one of them is there.
+    # torch.optim.Optimizer wraps the step of its classes in a profiler's range and the calls of registered hooks: 6 us where there is neither, as much as all else that the
+    # host does for four small tensors.  So the wrapped step is called where one of them is there.
     _wrapped_step = torch.optim.Optimizer.profile_hook_step(_step)
 
     def step(self, closure=None):

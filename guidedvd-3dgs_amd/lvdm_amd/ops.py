@@ -426,7 +426,8 @@ def relative_bias_attention(q, k, v, table, heads, *, max_distance=128, bidirect
     kv_lens int32 [B]: keys and values at and behind it are not seen, whatever they hold (their gradients are zeros); 0 is a length.  Rows of k and v before it
         have to be finite also where causal hides them from some queries.
     A query that sees nothing gives zeros and has no gradient, whatever the gradient of its output holds.  scale: default 64 ** -0.5.  Weights and their gradients pass through the inputs' 16 bits on their way into
-        the second products: in fp16 scale a loss whose gradients are small, as for any fp16 backward.  First derivatives only."""
+        the second products: in fp16 scale a loss whose gradients are small, as for any fp16 backward.  (Where gradients are wanted a row's weights are summed before that rounding, otherwise
+        behind it: outputs differ in last bits.)  First derivatives only; tangents are refused.  In a capture, no graph of the same leaves may live that was made outside it."""
     global _relative
     if _relative is None:
         from . import relative as _relative

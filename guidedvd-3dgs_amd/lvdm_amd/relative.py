@@ -33,7 +33,7 @@ def lib():
 
 
 def ext():
-    """The compiled operator (csrc/relattn_torch_ext.cpp: forward and backward as one torch::autograd::Function) over the same library instance."""
+    """The compiled operator (csrc/relattn_torch_ext.cpp: forward and backward as one node of the graph) over the same library instance."""
     global _EXT
     if _EXT is None:
         lib()
